@@ -39,6 +39,8 @@ extern "C" {
 /* quantised element types */
 #define T8G_QUANT_INT8 0            /* int8, scale = amax / 127, round half to even, clamp +-127 */
 #define T8G_QUANT_FP8_E4M3 1        /* float8_e4m3fn, scale = amax / 448, RNE, clamp +-448 */
+#define T8G_QUANT_MXFP4 2           /* e2m1, e8m0 scale per 32 (the _fp4 entry points only) */
+#define T8G_QUANT_NVFP4 3           /* e2m1, e4m3 scale per 16 and a row scale (the _fp4 entry points only) */
 
 /* Library version string, e.g. "0.1.0". */
 const char* t8g_version(void);
@@ -257,6 +259,75 @@ int t8g_rms_mod_quant_tensorwise_noalloc(const void* x, int64_t ld_x, const void
                                          int64_t rows_per_mod, int scale_is_multiplier, float eps, void* q,
                                          int64_t ld_q, void* res, int64_t ld_res, float* scale_out, int64_t S,
                                          int64_t D, int quant_kind, void* stream);
+
+/*
+ * ---- Microscaled 4-bit floating point --------------------------------------------------------
+ * A 4-bit matrix [rows, K] is three buffers:
+ *   q        e2m1 codes, two a byte (even k in the low half); row pitch ld_q in BYTES, a multiple
+ *            of 16; 16-byte aligned
+ *   sf       block scales in tiles of 128 rows x 4 blocks (512 bytes; row r, block b of a tile at byte
+ *            (r % 32) * 16 + (r / 32) * 4 + b), a row group's tiles consecutive along K;
+ *            t8g_fp4_scale_bytes(rows, K, kind) bytes, 16-byte aligned.  A caller that fills it
+ *            itself sets the scales of blocks past the row's last one (up to a multiple of 4) to 0.
+ *   scale    float32 [rows] (weights: numel 1 or rows), or NULL for 1
+ * and a value is code * block scale * row scale.
+ *   T8G_QUANT_MXFP4  blocks of 32, e8m0 scales (the quantisers write no row scale)
+ *   T8G_QUANT_NVFP4  blocks of 16, e4m3 scales, and a row scale that the quantisers make a power of
+ *                    two: 2^r, the least r >= -100 with amax(row) <= 6 * 448 * 2^r
+ * K is a multiple of 8; the last block of a row may be cut off.  No counterpart in the reference,
+ * whose quantised linears are int8 and fp8.
+ */
+
+/* Bytes of the block scales of a [rows, K] matrix; -1 for a negative size or another kind. */
+int64_t t8g_fp4_scale_bytes(int64_t rows, int64_t K, int quant_kind);
+
+/*
+ * Quantisation of a bf16 matrix: mxfp4 block scale = 2^(floor(log2(amax)) - 2) (at least 2^-127),
+ * nvfp4 block scale = e4m3(amax / (6 * 2^r)); code = e2m1(x / scale), to nearest, ties to even,
+ * saturating at 6.  A block (mxfp4) or row (nvfp4) that holds a NaN or an infinity gets a NaN scale.
+ *   x [S, D] bf16 (ld_x), q and sf as above, q_scale [S] float32 (NULL for mxfp4).
+ * The scales of rows S .. next multiple of 128 are written as 0.
+ * Requirements: D a multiple of 8, D <= 49152; x 16-byte aligned, ld_x a multiple of 8.
+ */
+int t8g_quant_rows_fp4(const void* x, int64_t ld_x, void* q, int64_t ld_q, void* sf, float* q_scale, int64_t S,
+                       int64_t D, int quant_kind, void* stream);
+
+/* The inverse: out[m, k] = cast((code * block scale) * q_scale[m]) in out_dtype (T8G_OUT_*); q_scale
+ * may be NULL (1).  out 16-byte aligned, ld_out >= D a multiple of 8. */
+int t8g_dequant_rows_fp4(const void* q, int64_t ld_q, const void* sf, const float* q_scale, void* out, int out_dtype,
+                         int64_t ld_out, int64_t S, int64_t D, int quant_kind, void* stream);
+
+/* t8g_rms_mod_quant with 4-bit output: t8g_quant_rows_fp4 of its bf16(h), bit for bit. */
+int t8g_rms_mod_quant_fp4(const void* x, int64_t ld_x, const void* w, const void* shift, const void* scale,
+                          int64_t ld_mod, const int32_t* mod_index, int64_t rows_per_mod, int scale_is_multiplier,
+                          float eps, void* q, int64_t ld_q, void* sf, float* q_scale, int64_t S, int64_t D,
+                          int quant_kind, void* stream);
+
+/* t8g_swiglu_quant with 4-bit output: t8g_quant_rows_fp4 of its bf16 act, bit for bit. */
+int t8g_swiglu_quant_fp4(const void* gate, const void* up, int64_t ld_in, void* q, int64_t ld_q, void* sf,
+                         float* q_scale, int64_t M, int64_t F, int quant_kind, void* stream);
+
+/*
+ * out[m, n] = cast( ((acc[m, n] * x_scale[m]) * w_scale[n or 0]) + float(bias[n]) )
+ * acc[m, n] = sum over blocks of x_sf * w_sf * sum_k x[m, k] * w[n, k], accumulated in float32
+ *   x [M, K], w [N, K] 4-bit matrices of one kind (ld_x, ld_w bytes); x_scale [M] or NULL; w_scale numel
+ *   1 or N, or NULL; bias numel 0 or N in the output type; out [M, N] of out_dtype, ld_out elements.
+ * Requirements: K >= 8; out 16-byte aligned, ld_out * element size a multiple of 16.  M == 0 or N == 0
+ * is a no-op.
+ */
+int t8g_gemm_fp4(const void* x, const void* x_sf, const float* x_scale, const void* w, const void* w_sf,
+                 const float* w_scale, int64_t w_scale_numel, const void* bias, int64_t bias_numel, void* out,
+                 int out_dtype, int64_t M, int64_t N, int64_t K, int64_t ld_x, int64_t ld_w, int64_t ld_out,
+                 int quant_kind, void* stream);
+
+/* t8g_gemm_fp4 as a gated residual: out = bf16(res + gate[g, n] * y), y the float32 value that t8g_gemm_fp4
+ * casts (one rounding, where t8g_gemm_i8_gated keeps torch's three).  N a multiple of 8; res, gate,
+ * gate_index, rows_per_gate and out as in t8g_gemm_i8_gated. */
+int t8g_gemm_fp4_gated(const void* x, const void* x_sf, const float* x_scale, const void* w, const void* w_sf,
+                       const float* w_scale, int64_t w_scale_numel, const void* bias, int64_t bias_numel,
+                       const void* res, int64_t ld_res, const void* gate, int64_t ld_gate, const int32_t* gate_index,
+                       int64_t rows_per_gate, void* out, int64_t M, int64_t N, int64_t K, int64_t ld_x, int64_t ld_w,
+                       int64_t ld_out, int quant_kind, void* stream);
 
 /* Bounded-wait self-test: one kernel waits `limit_ns` on an mbarrier that nothing
  * completes, gives up, records status 0x1FF and writes 1 to the device int *gave_up.

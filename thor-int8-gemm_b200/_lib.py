@@ -19,7 +19,7 @@ T8G_ERR_UNSUPPORTED = 2
 T8G_ERR_CUDA = 3
 
 OUT_BF16, OUT_F16, OUT_F32 = 0, 1, 2
-QUANT_INT8, QUANT_FP8_E4M3 = 0, 1
+QUANT_INT8, QUANT_FP8_E4M3, QUANT_MXFP4, QUANT_NVFP4 = 0, 1, 2, 3
 
 _vp, _i64, _i32, _u64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_uint64
 _f32 = ctypes.c_float
@@ -55,6 +55,16 @@ SIGNATURES = {
     "t8g_swiglu_quant_tensorwise": (_i32, [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _vp]),
     "t8g_rms_mod_quant_tensorwise_noalloc": (_i32, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i32, _f32,
                                                     _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i32, _vp]),
+    "t8g_fp4_scale_bytes": (_i64, [_i64, _i64, _i32]),
+    "t8g_quant_rows_fp4": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "t8g_dequant_rows_fp4": (_i32, [_vp, _i64, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _vp]),
+    "t8g_rms_mod_quant_fp4": (_i32, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i32, _f32,
+                                     _vp, _i64, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "t8g_swiglu_quant_fp4": (_i32, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "t8g_gemm_fp4": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i32,
+                            _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp]),
+    "t8g_gemm_fp4_gated": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64,
+                                  _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp]),
     "t8g_wait_selftest": (_i32, [_u64, _vp, _vp]),
 }
 

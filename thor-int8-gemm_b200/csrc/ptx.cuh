@@ -393,4 +393,70 @@ __host__ __device__ constexpr uint32_t make_idesc(uint32_t d_fmt, uint32_t a_fmt
          (static_cast<uint32_t>(M >> 4) << 24);
 }
 
+
+// ---------------------------------------------------------------------------
+// Block-scaled 4-bit products (kind::mxf4, e8m0 scale per 32 elements, and kind::mxf4nvf4 with
+// an e4m3 scale per 16): one instruction covers K = 64 (32 bytes of packed e2m1 per row).  The
+// scales are read from TMEM: row r of a 128-row group in lane r % 32 (repeated in all four
+// 32-lane groups), column r / 32, one 32-bit word of four consecutive block scales.
+// ---------------------------------------------------------------------------
+
+// Instruction descriptor: both operands e2m1, K-major, f32 accumulation.
+//   bits 4-5 / 29-30 first scale byte of the word for B / A (0 or 2, e8m0 only)
+//   bits 7-9 / 10-12 A / B format (1 = e2m1)   bits 17-22 N >> 3
+//   bit 23 scale type (0 = ue4m3, 1 = ue8m0)   bits 27-28 M >> 7
+__host__ __device__ constexpr uint32_t make_idesc_fp4(bool e8m0, int M, int N) {
+  return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(e8m0) << 23) |
+         (static_cast<uint32_t>(M >> 7) << 27);
+}
+
+// D[tmem] (+)= (A * SA) (B * SB)^T; MX: mxfp4, else nvfp4; PAIR: both CTAs' operands, M = 256.
+template <bool MX, bool PAIR>
+__device__ __forceinline__ void mma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sa,
+                                        uint32_t sb, uint32_t accumulate) {
+#define T8G_MMA_FP4(GROUP, KIND)                                                                                  \
+  asm volatile(                                                                                                  \
+      "{\n"                                                                                                      \
+      "  .reg .pred p;\n"                                                                                        \
+      "  setp.ne.b32 p, %6, 0;\n"                                                                                \
+      "  tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p;\n"                      \
+      "}\n" ::"r"(d_tmem),                                                                                       \
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)                                    \
+      : "memory")
+  if constexpr (MX && PAIR) T8G_MMA_FP4("2", "mxf4.block_scale.scale_vec::2X");
+  if constexpr (MX && !PAIR) T8G_MMA_FP4("1", "mxf4.block_scale.scale_vec::2X");
+  if constexpr (!MX && PAIR) T8G_MMA_FP4("2", "mxf4nvf4.block_scale.scale_vec::4X");
+  if constexpr (!MX && !PAIR) T8G_MMA_FP4("1", "mxf4nvf4.block_scale.scale_vec::4X");
+#undef T8G_MMA_FP4
+}
+
+// 32 rows x 16 bytes of shared memory (512 contiguous bytes) -> four TMEM columns, the same
+// 32 lanes in each of the four lane groups; PAIR: in both CTAs, each from its own memory.
+// Executed in issue order with the MMAs of the same thread.
+template <bool PAIR>
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t s_desc) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(s_desc) : "memory");
+}
+
+// Shared-memory matrix descriptor of such a 512-byte tile: 16-byte rows, no swizzle, 8-row
+// groups 128 bytes apart (fields as in smem_desc_k_sw128).
+__device__ __forceinline__ uint64_t smem_desc_scales(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFF);
+  d |= static_cast<uint64_t>(128 >> 4) << 16;
+  d |= static_cast<uint64_t>(128 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  return d;
+}
+
+// A float at `addr`, an address of the cluster's shared memory (mapa_shared).
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 }  // namespace t8g

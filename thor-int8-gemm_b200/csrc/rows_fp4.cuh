@@ -1,0 +1,400 @@
+// Row kernels of the microscaled 4-bit formats (HBM-bound): quantisation of bf16 rows, RMSNorm +
+// modulation + quantisation, SwiGLU + quantisation, and the inverse.
+//
+// e2m1 values 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign, rounded to nearest (ties to the even
+// code), saturating at 6; two codes a byte, the even column in the low half.
+//   mxfp4: block of 32, scale 2^(floor(log2 amax) - 2), stored as its exponent + 127 (e8m0), at
+//          least 0: from the bf16 exponent field e of amax it is max(e - 2, 0);
+//   nvfp4: block of 16, row scale 2^r with the least r >= -100 that has amax(row) <= 6 * 448 * 2^r,
+//          block scale e4m3(amax / (6 * 2^r)).
+// The values quantised are bf16 (8 significant bits), also behind a norm or a SwiGLU, so that the
+// fused forms give exactly what quantising their stored bf16 result gives.  Every decision is
+// then exact in fp32: mxfp4's x / scale is a shift; for nvfp4 x / scale either is one of the seven
+// borders between e2m1 values or at least 2^-10 away from it (x and border * scale are both
+// integers of at most 8 bits on a common grid), so a quotient rounded to a multiple of 2^-14, which the fp32 adder does
+// (add and subtract 1.5 * 2^9), falls on the border exactly when x does.
+// A block with a NaN or an infinity has a NaN scale; a row with one has (nvfp4) a NaN row scale,
+// so every product with that row is NaN.
+//
+// Scales are stored in tiles of 128 rows x 4 blocks (gemm_fp4.cuh); rows past the last one, up to a
+// multiple of 128, and blocks past the last one, up to a multiple of 4, are written as 0.
+#pragma once
+
+#include "rows.cuh"
+
+namespace t8g {
+namespace rows {
+
+struct Fp4Out {
+  uint8_t* q;        // [S, D / 2]
+  int64_t ld_q;      // bytes
+  uint8_t* sf;       // scale tiles
+  float* q_scale;    // [S], nvfp4 only
+  int64_t S;
+  int words;         // 4-block scale words of a row
+};
+
+// Address of scale word 0 of a row; word w is 512 * w bytes on.
+__host__ __device__ __forceinline__ int64_t scale_row(int64_t row, int words) {
+  return (row >> 7) * words * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
+}
+
+// Largest magnitude of eight bf16 values as bf16 bits (integer order: NaN above infinity above
+// every number).
+__device__ __forceinline__ uint32_t absmax_bits(const uint4& u) {
+  const uint32_t m = max_u16x2(max_u16x2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu),
+                               max_u16x2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
+  return max(m & 0xFFFFu, m >> 16);
+}
+__device__ __forceinline__ uint32_t warp_max_u32(uint32_t v) {
+  uint32_t r;
+  asm volatile("redux.sync.max.u32 %0, %1, 0xffffffff;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// nvfp4: the row scale 2^r from the row's largest magnitude (bf16 bits) and its inverse (0 for a row
+// with a NaN or an infinity, whose scale is NaN).
+__device__ __forceinline__ float row_scale_fp4(uint32_t amax, float* inverse) {
+  if (amax >= 0x7F80u) {
+    *inverse = 0.f;
+    return __uint_as_float(0x7FC00000u);
+  }
+  // 6 * 448 = 1.3125 * 2^11, and 0.3125 is 40 / 128
+  const int r = max(static_cast<int>(amax >> 7) - 127 - 11 + ((amax & 0x7Fu) > 40u ? 1 : 0), -100);
+  *inverse = __uint_as_float(static_cast<uint32_t>(127 - r) << 23);
+  return __uint_as_float(static_cast<uint32_t>(127 + r) << 23);
+}
+
+// Eight fp32 values -> eight e2m1 codes (first value in the lowest four bits).
+__device__ __forceinline__ uint32_t cvt_e2m1x8(const float2 (&v)[4]) {
+  uint32_t r;
+  asm("{ .reg .b8 a, b, c, d;\n"
+      "  cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n"
+      "  cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+      "  cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n"
+      "  cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+      "  mov.b32 %0, {a, b, c, d}; }"
+      : "=r"(r)
+      : "f"(v[0].x), "f"(v[0].y), "f"(v[1].x), "f"(v[1].y), "f"(v[2].x), "f"(v[2].y), "f"(v[3].x), "f"(v[3].y));
+  return r;
+}
+__device__ __forceinline__ float e4m3_to_f32(uint32_t byte) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(byte)));
+  return __half2float(__ushort_as_half(static_cast<uint16_t>(h & 0xFFFFu)));
+}
+__device__ __forceinline__ float rcp_approx(float v) {   // within 1 ulp; see the 2^-14 rounding above
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// One warp step: lane l holds vector c0 + l of a row (zeros past the row's end).  Returns the
+// eight codes and, in `word`, the four block scales of the lane's group of 16 (mxfp4) or 8
+// (nvfp4) lanes.  Every lane of the warp takes part.
+template <bool MX>
+__device__ __forceinline__ uint32_t quant_vec_fp4(const uint4& u, float row_inverse, uint32_t& word) {
+  const int lane = threadIdx.x & 31;
+  uint32_t b = absmax_bits(u);
+  b = max(b, __shfl_xor_sync(0xFFFFFFFFu, b, 1));
+  uint32_t byte;
+  float2 v[4];
+  unpack_pairs(u, v);
+  if constexpr (MX) {
+    b = max(b, __shfl_xor_sync(0xFFFFFFFFu, b, 2));
+    const int e = max(static_cast<int>(b >> 7) - 2, 0);
+    const bool finite = b < 0x7F80u;
+    byte = finite ? static_cast<uint32_t>(e) : 255u;
+    const float mult = finite ? __uint_as_float(static_cast<uint32_t>(254 - e) << 23) : 0.f;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) v[p] = mul2_rn(v[p], make_float2(mult, mult));
+    word = byte << (8 * ((lane >> 2) & 3));
+    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
+    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
+  } else {
+    // RN(t / 6) with one correction step (quant8 of rows.cuh), then e4m3
+    const float t = __fmul_rn(__uint_as_float(b << 16), row_inverse);
+    const float sixth = 1.0f / 6.0f;
+    const float q0 = __fmul_rn(t, sixth);
+    const float q1 = __fmaf_rn(__fmaf_rn(-6.0f, q0, t), sixth, q0);
+    byte = cvt_e4m3x2(q1, 0.f) & 0xFFu;
+    const float sb = e4m3_to_f32(byte);
+    const float mult = sb > 0.f ? __fmul_rn(row_inverse, rcp_approx(sb)) : 0.f;
+    const float2 mult2 = make_float2(mult, mult);
+    constexpr float kGrid = 768.f;   // 1.5 * 2^9: one ulp is 2^-14
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const float2 y = fma2_rn(v[p], mult2, make_float2(kGrid, kGrid));
+      v[p] = make_float2(__fadd_rn(y.x, -kGrid), __fadd_rn(y.y, -kGrid));
+    }
+    word = byte << (8 * ((lane >> 1) & 3));
+    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 2);
+    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
+  }
+  return cvt_e2m1x8(v);
+}
+
+// Vectors c0 + lane (a multiple of 32 apart) of row `row`, held in u: codes and scale words.
+template <bool MX>
+__device__ __forceinline__ void store_vec_fp4(const Fp4Out& o, uint8_t* qrow, uint8_t* sfrow, int c, int nvec,
+                                              const uint4& u, float row_inverse) {
+  constexpr int kLanesPerWord = MX ? 16 : 8;
+  uint32_t word;
+  const uint32_t codes = quant_vec_fp4<MX>(u, row_inverse, word);
+  if (c < nvec) {
+    *reinterpret_cast<uint32_t*>(qrow + 4 * c) = codes;
+    if ((c & (kLanesPerWord - 1)) == 0)
+      *reinterpret_cast<uint32_t*>(sfrow + 512 * static_cast<int64_t>(c / kLanesPerWord)) = word;
+  }
+}
+
+// Scale words of the rows that fill up the last tile: zeros, dealt over the grid's warps.
+__device__ __forceinline__ void zero_pad_rows(const Fp4Out& o) {
+  const int64_t end = (o.S + 127) & ~static_cast<int64_t>(127);
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+  for (int64_t row = o.S + static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); row < end;
+       row += warps)
+    for (int w = threadIdx.x & 31; w < o.words; w += 32)
+      *reinterpret_cast<uint32_t*>(o.sf + scale_row(row, o.words) + 512 * static_cast<int64_t>(w)) = 0u;
+}
+
+// ---------------------------------------------------------------- quantisation
+// One row per warp (rows of at most kWarpRowMaxBytes).
+template <bool MX>
+__global__ void __launch_bounds__(1024) quant_rows_fp4_warp_kernel(const QuantRowsArgs a, const WarpRingGeom g,
+                                                                   const Fp4Out o) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int lane = threadIdx.x & 31;
+  const int nvec = a.D >> 3;
+  auto src = [&](int64_t r) -> const void* { return a.x + r * a.ld_x; };
+  warp_row_loop(smem, g, a.S, src, [&](int64_t row, const uint8_t* slot) {
+    float inverse = 0.f;
+    if constexpr (!MX) {
+      uint32_t m = 0;
+      for (int c = lane; c < nvec; c += 32) m = max(m, absmax_bits(lds_v4(slot + 16 * c)));
+      const float scale = row_scale_fp4(warp_max_u32(m), &inverse);
+      if (lane == 0) o.q_scale[row] = scale;
+    }
+    uint8_t* qrow = o.q + row * o.ld_q;
+    uint8_t* sfrow = o.sf + scale_row(row, o.words);
+    for (int c = lane; c - lane < nvec; c += 32)
+      store_vec_fp4<MX>(o, qrow, sfrow, c, nvec, c < nvec ? lds_v4(slot + 16 * c) : make_uint4(0, 0, 0, 0), inverse);
+  });
+  zero_pad_rows(o);
+}
+
+// Row maximum (bf16 bits) over a row group.
+__device__ __forceinline__ uint32_t group_max_u32(const RowGroup& grp, uint32_t v, float* red) {
+  v = warp_max_u32(v);
+  if (grp.T == 32) return v;
+  const int lane = grp.t & 31;
+  if (lane == 0) red[grp.t >> 5] = __uint_as_float(v);
+  group_sync(grp);
+  return warp_max_u32(lane < (grp.T >> 5) ? __float_as_uint(red[lane]) : 0u);
+}
+
+// The quantising pass of a row group over bf16 vectors in its slot.
+template <bool MX>
+__device__ __forceinline__ void group_quant_fp4(const RowGroup& grp, const Fp4Out& o, int64_t row, const uint8_t* slot,
+                                                int nvec, float inverse) {
+  uint8_t* qrow = o.q + row * o.ld_q;
+  uint8_t* sfrow = o.sf + scale_row(row, o.words);
+  const int lane = grp.t & 31;
+  for (int c = grp.t; c - lane < nvec; c += grp.T)
+    store_vec_fp4<MX>(o, qrow, sfrow, c, nvec, c < nvec ? lds_v4(slot + 16 * c) : make_uint4(0, 0, 0, 0), inverse);
+}
+
+// Longer rows: one CTA per row.
+template <bool MX>
+__global__ void __launch_bounds__(512) quant_rows_fp4_kernel(const QuantRowsArgs a, const RingGeom g, const Fp4Out o) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const RowGroup grp = row_group(blockDim.x);
+  const int nvec = a.D >> 3;
+  auto src = [&](int64_t r, int) -> const void* { return a.x + r * a.ld_x; };
+  row_loop(smem, g, grp, a.S, src, [&](int64_t row, const uint8_t* slot, const RingState& rs) {
+    float inverse = 0.f;
+    if constexpr (!MX) {
+      uint32_t m = 0;
+      for (int c = grp.t; c < nvec; c += grp.T) m = max(m, absmax_bits(lds_v4(slot + 16 * c)));
+      const float scale = row_scale_fp4(group_max_u32(grp, m, rs.red_max), &inverse);
+      if (grp.t == 0) o.q_scale[row] = scale;
+    }
+    group_quant_fp4<MX>(grp, o, row, slot, nvec, inverse);
+  });
+  zero_pad_rows(o);
+}
+
+// ---------------------------------------------------------------- RMSNorm + modulation
+// The norm of rms_mod_warp_kernel / rms_mod_kernel (the same sums in the same order: h is bit for
+// bit theirs), bf16(h) left in the slot and quantised from there.
+template <bool MX>
+__global__ void __launch_bounds__(1024) rms_mod_fp4_warp_kernel(const RmsArgs a, const WarpRingGeom g, const Fp4Out o,
+                                                                const int T) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int lane = threadIdx.x & 31;
+  const int nvec = a.D >> 3;
+  const int nw = T >> 5;
+  const float fD = static_cast<float>(a.D);
+  auto src = [&](int64_t r) -> const void* { return a.x + r * a.ld_x; };
+  warp_row_loop(smem, g, a.S, src, [&](int64_t row, uint8_t* slot) {
+    float ss = 0.f;
+    for (int j = 0; j < nw; ++j) {
+      float2 acc = make_float2(0.f, 0.f);
+      for (int c = 32 * j + lane; c < nvec; c += T) acc = row_sumsq_vec(acc, lds_v4(slot + 16 * c));
+      float v = __fadd_rn(acc.x, acc.y);
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xFFFFFFFFu, v, off));
+      ss = j == 0 ? v : __fadd_rn(ss, v);
+    }
+    const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, fD), a.eps)));
+    const int64_t m = a.mod_index ? static_cast<int64_t>(__ldg(a.mod_index + row)) : row / a.rows_per_mod;
+    uint32_t mx = 0;
+    for (int c = lane; c < nvec; c += 32) {
+      float2 s[4], b[4], x[4], h[4];
+      load_mod8(a, m, c, s, b);
+      rms_h8(lds_v4(slot + 16 * c), make_float2(inv, inv), s, b, a.w, c, x, h);
+      const uint4 hu = make_uint4(f2_to_bf2(h[0]), f2_to_bf2(h[1]), f2_to_bf2(h[2]), f2_to_bf2(h[3]));
+      mx = max(mx, absmax_bits(hu));
+      *reinterpret_cast<uint4*>(slot + 16 * c) = hu;
+    }
+    float inverse = 0.f;
+    if constexpr (!MX) {
+      const float scale = row_scale_fp4(warp_max_u32(mx), &inverse);
+      if (lane == 0) o.q_scale[row] = scale;
+    }
+    uint8_t* qrow = o.q + row * o.ld_q;
+    uint8_t* sfrow = o.sf + scale_row(row, o.words);
+    for (int c = lane; c - lane < nvec; c += 32)   // every lane reads back what it wrote
+      store_vec_fp4<MX>(o, qrow, sfrow, c, nvec, c < nvec ? lds_v4(slot + 16 * c) : make_uint4(0, 0, 0, 0), inverse);
+  });
+  zero_pad_rows(o);
+}
+
+template <bool MX>
+__global__ void __launch_bounds__(512) rms_mod_fp4_kernel(const RmsArgs a, const RingGeom g, const Fp4Out o) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const RowGroup grp = row_group(blockDim.x);
+  const int nvec = a.D >> 3;
+  const float fD = static_cast<float>(a.D);
+  auto src = [&](int64_t r, int) -> const void* { return a.x + r * a.ld_x; };
+  row_loop(smem, g, grp, a.S, src, [&](int64_t row, uint8_t* slot, const RingState& rs) {
+    float2 acc = make_float2(0.f, 0.f);
+    for (int c = grp.t; c < nvec; c += grp.T) acc = row_sumsq_vec(acc, lds_v4(slot + 16 * c));
+    const float ss = block_sum(grp, __fadd_rn(acc.x, acc.y), rs.red_sum);
+    const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, fD), a.eps)));
+    const int64_t m = a.mod_index ? static_cast<int64_t>(__ldg(a.mod_index + row)) : row / a.rows_per_mod;
+    uint32_t mx = 0;
+    for (int c = grp.t; c < nvec; c += grp.T) {
+      float2 s[4], b[4], x[4], h[4];
+      load_mod8(a, m, c, s, b);
+      rms_h8(lds_v4(slot + 16 * c), make_float2(inv, inv), s, b, a.w, c, x, h);
+      const uint4 hu = make_uint4(f2_to_bf2(h[0]), f2_to_bf2(h[1]), f2_to_bf2(h[2]), f2_to_bf2(h[3]));
+      mx = max(mx, absmax_bits(hu));
+      *reinterpret_cast<uint4*>(slot + 16 * c) = hu;
+    }
+    slot_written();
+    float inverse = 0.f;
+    if constexpr (!MX) {
+      const float scale = row_scale_fp4(group_max_u32(grp, mx, rs.red_max), &inverse);
+      if (grp.t == 0) o.q_scale[row] = scale;
+    }
+    group_quant_fp4<MX>(grp, o, row, slot, nvec, inverse);   // every thread reads back what it wrote
+  });
+  zero_pad_rows(o);
+}
+
+// ---------------------------------------------------------------- SwiGLU
+// act = bf16((gate * sigmoid(gate)) * up) as swiglu_kernel computes it, kept in the gate row's
+// slot and quantised from there.
+template <bool MX>
+__global__ void __launch_bounds__(1024) swiglu_fp4_kernel(const SwigluArgs a, const RingGeom g, const Fp4Out o,
+                                                          const int T) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  load_sigmoid_table(reinterpret_cast<uint32_t*>(smem), threadIdx.x, blockDim.x);
+  const uint32_t sig = smem_u32(smem);
+  __syncthreads();
+  const RowGroup grp = row_group(T);
+  uint8_t* ring = smem + kSigmoidBytes + static_cast<size_t>(grp.index) * ring_bytes(g);
+  const int nvec = a.F >> 3;
+  auto src = [&](int64_t r, int part) -> const void* { return (part ? a.up : a.gate) + r * a.ld_in; };
+  row_loop(ring, g, grp, a.M, src, [&](int64_t row, uint8_t* slot, const RingState& rs) {
+    const uint8_t* up = slot + g.part_bytes;
+    uint32_t mx = 0;
+    float unused = 0.f;
+    for (int c = grp.t; c < nvec; c += T) {
+      const uint4 au = swiglu8(slot, up, c, sig, unused, false);
+      mx = max(mx, absmax_bits(au));
+      *reinterpret_cast<uint4*>(slot + 16 * c) = au;
+    }
+    slot_written();
+    float inverse = 0.f;
+    if constexpr (!MX) {
+      const float scale = row_scale_fp4(group_max_u32(grp, mx, rs.red_max), &inverse);
+      if (grp.t == 0) o.q_scale[row] = scale;
+    }
+    group_quant_fp4<MX>(grp, o, row, slot, nvec, inverse);   // every thread reads back what it wrote
+  });
+  zero_pad_rows(o);
+}
+
+// ---------------------------------------------------------------- inverse
+// out[m, k] = cast((code * block scale) * row scale), one vector of eight values per thread.
+// OUT: 0 bf16, 1 fp16, 2 fp32.
+struct DequantFp4Args {
+  const uint8_t* q;
+  int64_t ld_q;
+  const uint8_t* sf;
+  const float* q_scale;   // or null (1)
+  void* out;
+  int64_t ld_out;
+  int64_t S;
+  int D;
+  int words;
+};
+
+template <bool MX, int OUT>
+__global__ void __launch_bounds__(256) dequant_rows_fp4_kernel(const DequantFp4Args a) {
+  const int nvec = a.D >> 3;
+  const int64_t total = a.S * nvec;
+  const int64_t G = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += G) {
+    const int64_t row = i / nvec;
+    const int c = static_cast<int>(i - row * nvec);
+    const uint32_t codes = __ldg(reinterpret_cast<const uint32_t*>(a.q + row * a.ld_q + 4 * c));
+    const int block = MX ? c >> 2 : c >> 1;
+    const uint32_t byte = __ldg(a.sf + scale_row(row, a.words) + 512 * static_cast<int64_t>(block >> 2) + (block & 3));
+    const float rs = a.q_scale ? __ldg(a.q_scale + row) : 1.f;
+    const float sb = MX ? __uint_as_float(byte == 255u ? 0x7FC00000u : byte == 0u ? 0x00400000u : byte << 23)
+                        : e4m3_to_f32(byte);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      // e2m1: two exponent bits (bias 1), one mantissa bit
+      const uint32_t code = codes >> (4 * j);
+      const uint32_t mag = code & 7u;
+      const float e = mag < 2u ? 0.5f * static_cast<float>(mag)
+                               : __uint_as_float(((126u + (mag >> 1)) << 23) | ((mag & 1u) << 22));
+      v[j] = __fmul_rn(__fmul_rn((code & 8u) ? -e : e, sb), rs);
+    }
+    if constexpr (OUT == 2) {
+      float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * a.ld_out + 8 * c);
+      p[0] = make_float4(v[0], v[1], v[2], v[3]);
+      p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        if constexpr (OUT == 0) {
+          w[p] = pack_bf16(v[2 * p], v[2 * p + 1]);
+        } else {
+          const __half2 h = __floats2half2_rn(v[2 * p], v[2 * p + 1]);
+          w[p] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.ld_out + 8 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+}  // namespace rows
+}  // namespace t8g

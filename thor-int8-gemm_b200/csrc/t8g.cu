@@ -15,8 +15,10 @@
 
 #include "../../include/thor_int8_gemm_b200.h"
 #include "gemm.cuh"
+#include "gemm_fp4.cuh"
 #include "ptx.cuh"
 #include "rows.cuh"
+#include "rows_fp4.cuh"
 
 namespace {
 
@@ -583,9 +585,9 @@ int ensure_row_attr(K kern, int dev) {
   return T8G_OK;
 }
 
-template <typename K, typename A>
+template <typename K, typename A, typename... Extra>
 int launch_rows(K kern, int T, const A& args, t8g::rows::RingGeom g, int64_t rows, int dev, int sms, cudaStream_t st,
-                const char* what) {
+                const char* what, Extra... extra) {
   using t8g::rows::kMaxStages;
   using t8g::rows::kRingHeader;
   int rc = ensure_row_attr(kern, dev);
@@ -606,7 +608,7 @@ int launch_rows(K kern, int T, const A& args, t8g::rows::RingGeom g, int64_t row
   if (occ < 1) occ = 1;
   const int64_t cap = static_cast<int64_t>(sms) * occ;
   const unsigned grid = static_cast<unsigned>(rows < cap ? rows : cap);
-  kern<<<grid, T, smem, st>>>(args, g);
+  kern<<<grid, T, smem, st>>>(args, g, extra...);
   T8G_CHECK_CUDA(cudaGetLastError(), what);
   return T8G_OK;
 }
@@ -654,9 +656,9 @@ int launch_warp_rows(K kern, const A& args, uint32_t row_bytes, int64_t rows, in
 // Launch the SwiGLU kernel: one CTA per SM holding the 32 KB sigmoid table and up to eight
 // row groups of T threads (at most 1024 threads), each with a ring of as many slots (>= 2)
 // as the rest of the CTA's shared memory holds.
-template <typename K>
+template <typename K, typename... Extra>
 int launch_swiglu(K kern, int T, const t8g::rows::SwigluArgs& args, t8g::rows::RingGeom g, int64_t rows, int dev,
-                  int sms, cudaStream_t st, const char* what) {
+                  int sms, cudaStream_t st, const char* what, Extra... extra) {
   using namespace t8g::rows;
   int rc = ensure_row_attr(kern, dev);
   if (rc) return rc;
@@ -680,7 +682,7 @@ int launch_swiglu(K kern, int T, const t8g::rows::SwigluArgs& args, t8g::rows::R
   const int64_t want = (rows + groups - 1) / groups;
   const int64_t cap = static_cast<int64_t>(sms) * occ;
   const unsigned grid = static_cast<unsigned>(want < cap ? want : cap);
-  kern<<<grid, threads, smem, st>>>(args, g, T);
+  kern<<<grid, threads, smem, st>>>(args, g, extra..., T);
   T8G_CHECK_CUDA(cudaGetLastError(), what);
   return T8G_OK;
 }
@@ -1266,3 +1268,5 @@ int t8g_wait_selftest(uint64_t limit_ns, int* gave_up, void* stream) {
 }
 
 }  // extern "C"
+
+#include "t8g_fp4.cuh"

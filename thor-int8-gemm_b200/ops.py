@@ -468,6 +468,276 @@ def swiglu_quant_tensorwise(gate, up, kind="fp8_e4m3", stream=None):
     return q, qs, act
 
 
+# ---------------------------------------------------------------- microscaled 4-bit formats
+# A 4-bit matrix [S, D] is (q, sf, q_scale): q uint8 [S, D / 2], two e2m1 codes a byte (the even column in
+# the low half) at a row pitch that is a multiple of 16 bytes; sf uint8, the block scales in tiles of
+# 128 rows x 4 blocks (`fp4_scale_rows` gives them row by row); q_scale float32 [S], or None (mxfp4).
+FP4_CODE = {"mxfp4": _lib.QUANT_MXFP4, "nvfp4": _lib.QUANT_NVFP4}
+FP4_BLOCK = {"mxfp4": 32, "nvfp4": 16}
+
+
+def _fp4_code(kind: str) -> int:
+    if kind not in FP4_CODE:
+        raise ValueError(f"kind {kind!r} is not a 4-bit format ({', '.join(FP4_CODE)})")
+    return FP4_CODE[kind]
+
+
+def fp4_scale_bytes(rows: int, D: int, kind: str) -> int:
+    """Bytes of the block scales of a [rows, D] 4-bit matrix."""
+    n = _lib.load().t8g_fp4_scale_bytes(rows, D, _fp4_code(kind))
+    if n < 0:
+        raise ValueError(f"bad sizes {rows} x {D}")
+    return n
+
+
+def fp4_scale_rows(sf: torch.Tensor, rows: int, D: int, kind: str) -> torch.Tensor:
+    """The block scales as a [rows, ceil(D / block)] uint8 matrix (e8m0 or e4m3 bytes)."""
+    _fp4_code(kind)
+    blocks = -(-D // FP4_BLOCK[kind])
+    groups = -(-rows // 128)
+    t = sf[:fp4_scale_bytes(rows, D, kind)].view(groups, -(-blocks // 4), 32, 4, 4)
+    return t.permute(0, 3, 2, 1, 4).reshape(groups * 128, -1)[:rows, :blocks]
+
+
+def _fp4_empty(S: int, D: int, kind: str, device):
+    q = torch.empty(S, -(-D // 32) * 16, dtype=torch.uint8, device=device)[:, :D // 2]
+    sf = torch.empty(fp4_scale_bytes(S, D, kind), dtype=torch.uint8, device=device)
+    q_scale = torch.empty(S, dtype=torch.float32, device=device) if kind == "nvfp4" else None
+    return q, sf, q_scale
+
+
+def _pitch(t: torch.Tensor, multiple: int) -> int:
+    """Row stride in elements; a single row has none of its own."""
+    if t.shape[0] > 1:
+        return t.stride(0)
+    return -(-t.shape[1] // multiple) * multiple
+
+
+def _one_device(**tensors) -> None:
+    seen = {n: t.get_device() for n, t in tensors.items() if t is not None}
+    if len(set(seen.values())) > 1:
+        raise ValueError(f"tensors on different CUDA devices: {seen}")
+
+
+def _fp4_operand(name: str, q: torch.Tensor, sf: torch.Tensor, kind: str):
+    _need_cuda(name, q, torch.uint8, 2)
+    rows, D = q.shape[0], 2 * q.shape[1]
+    _need_cuda(f"{name}_sf", sf, torch.uint8, 1)
+    if not sf.is_contiguous() or sf.numel() < fp4_scale_bytes(rows, D, kind):
+        raise ValueError(f"{name}_sf must be contiguous with at least {fp4_scale_bytes(rows, D, kind)} bytes "
+                         f"({kind}, {rows} x {D}), got {sf.numel()}")
+    return rows, D
+
+
+def _fp4_row_len(name: str, D: int) -> None:
+    if D % 8:
+        raise ValueError(f"{name} has rows of {D} elements, not a multiple of 8")
+
+
+def quant_rows_fp4(x: torch.Tensor, kind: str = "nvfp4", stream=None):
+    """4-bit quantisation of a bf16 [S, D] matrix (D a multiple of 8) -> (q, sf, q_scale).
+
+    mxfp4: blocks of 32 with a power-of-two scale, q_scale None; nvfp4: blocks of 16 with an
+    e4m3 scale, and a power of two per row.  A block (mxfp4) or row (nvfp4) that holds a NaN or an
+    infinity stands for NaN."""
+    code = _fp4_code(kind)
+    _need_cuda("x", x, torch.bfloat16, 2)
+    S, D = x.shape
+    _fp4_row_len("x", D)
+    q, sf, q_scale = _fp4_empty(S, D, kind, x.device)
+    with _on(x.device):
+        rc = _lib.load().t8g_quant_rows_fp4(_ptr(x), _pitch(x, 8), _ptr(q), _pitch(q, 16), _ptr(sf), _ptr(q_scale), S, D,
+                                            code, _stream_handle(x.device, stream))
+    _lib.check(rc)
+    return q, sf, q_scale
+
+
+def dequant_rows_fp4(q: torch.Tensor, sf: torch.Tensor, q_scale: torch.Tensor | None = None, kind: str = "nvfp4",
+                     out_dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
+    """What a 4-bit matrix stands for: (code * block scale) * q_scale as bf16, fp16 or fp32 [S, D]."""
+    code = _fp4_code(kind)
+    S, D = _fp4_operand("q", q, sf, kind)
+    _fp4_row_len("q", D)
+    if q_scale is not None:
+        _need_cuda("q_scale", q_scale, torch.float32, 1)
+        if q_scale.numel() != S or not q_scale.is_contiguous():
+            raise ValueError("q_scale must be a contiguous float32 tensor with S elements")
+    if out_dtype not in OUT_CODE:
+        raise TypeError(f"out_dtype {out_dtype} is not one of {tuple(OUT_CODE)}")
+    _one_device(q=q, sf=sf, q_scale=q_scale)
+    out = torch.empty(S, D, dtype=out_dtype, device=q.device)
+    with _on(q.device):
+        rc = _lib.load().t8g_dequant_rows_fp4(_ptr(q), _pitch(q, 16), _ptr(sf), _ptr(q_scale), _ptr(out),
+                                              OUT_CODE[out_dtype], D, S, D, code, _stream_handle(q.device, stream))
+    _lib.check(rc)
+    return out
+
+
+def rms_mod_quant_fp4(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, *, w: torch.Tensor | None = None,
+                      mod_index: torch.Tensor | None = None, rows_per_mod: int | None = None,
+                      scale_is_multiplier: bool = False, eps: float = 1e-6, kind: str = "nvfp4", stream=None):
+    """rms_mod_quant with 4-bit output -> (q, sf, q_scale): quant_rows_fp4 of its bf16 h, bit for
+    bit, without storing h.  Values of mod_index are trusted to be rows of shift / scale."""
+    code = _fp4_code(kind)
+    _need_cuda("x", x, torch.bfloat16, 2)
+    S, D = x.shape
+    _fp4_row_len("x", D)
+    shift2, scale2, rpm = _mod_args(x, shift, scale, mod_index, rows_per_mod)
+    if shift2.shape[0] != scale2.shape[0]:
+        raise ValueError(f"shift has {shift2.shape[0]} rows, scale {scale2.shape[0]}")
+    if mod_index is None and (rpm < 1 or (S and (S - 1) // rpm >= shift2.shape[0])):
+        raise ValueError(f"rows_per_mod={rpm} maps rows past the {shift2.shape[0]} modulation rows")
+    if w is not None:
+        _need_cuda("w", w, torch.bfloat16, 1)
+        if w.numel() != D:
+            raise ValueError("w must have D elements")
+    _one_device(x=x, shift=shift, scale=scale, w=w, mod_index=mod_index)
+    q, sf, q_scale = _fp4_empty(S, D, kind, x.device)
+    with _on(x.device):
+        rc = _lib.load().t8g_rms_mod_quant_fp4(
+            _ptr(x), _pitch(x, 8), _ptr(w), _ptr(shift2), _ptr(scale2), _pitch(shift2, 8), _ptr(mod_index), rpm,
+            int(scale_is_multiplier), float(eps), _ptr(q), _pitch(q, 16), _ptr(sf), _ptr(q_scale), S, D, code,
+            _stream_handle(x.device, stream))
+    _lib.check(rc)
+    return q, sf, q_scale
+
+
+def swiglu_quant_fp4(gate: torch.Tensor, up: torch.Tensor, kind: str = "nvfp4", stream=None):
+    """swiglu_quant with 4-bit output -> (q, sf, q_scale): quant_rows_fp4 of act = bf16(silu(gate) *
+    up), bit for bit, without storing act."""
+    code = _fp4_code(kind)
+    _need_cuda("gate", gate, torch.bfloat16, 2)
+    _need_cuda("up", up, torch.bfloat16, 2)
+    M, F = gate.shape
+    if gate.shape != up.shape or (M > 1 and gate.stride(0) != up.stride(0)):
+        raise ValueError("gate and up must have the same shape and strides")
+    _fp4_row_len("gate", F)
+    _one_device(gate=gate, up=up)
+    q, sf, q_scale = _fp4_empty(M, F, kind, gate.device)
+    with _on(gate.device):
+        rc = _lib.load().t8g_swiglu_quant_fp4(_ptr(gate), _ptr(up), _pitch(gate, 8), _ptr(q), _pitch(q, 16), _ptr(sf),
+                                              _ptr(q_scale), M, F, code, _stream_handle(gate.device, stream))
+    _lib.check(rc)
+    return q, sf, q_scale
+
+
+def swiglu_quant_fp4_fc1(y: torch.Tensor, kind: str = "nvfp4", stream=None):
+    """swiglu_quant_fp4 of a [M, 2F] fc1 output whose first half is the gate."""
+    _need_cuda("y", y, torch.bfloat16, 2)
+    if y.shape[1] % 2:
+        raise ValueError(f"y must be [M, 2F], got {tuple(y.shape)}")
+    F = y.shape[-1] // 2
+    return swiglu_quant_fp4(y[:, :F], y[:, F:], kind=kind, stream=stream)
+
+
+def _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype):
+    """Argument rules of the 4-bit products -> (M, N, K, w_scale numel, bias numel)."""
+    M, K = _fp4_operand("x", x, x_sf, kind)
+    N, Kw = _fp4_operand("w", w, w_sf, kind)
+    if Kw != K:
+        raise ValueError(f"w has K={Kw}, x has K={K}")
+    if K < 8 or K % 8:
+        raise ValueError(f"K={K} must be a positive multiple of 8")
+    if x_scale is not None:
+        _need_cuda("x_scale", x_scale, torch.float32)
+        if x_scale.numel() != M or not x_scale.is_contiguous():
+            raise ValueError("x_scale must be a contiguous float32 tensor with M elements")
+    if w_scale is not None:
+        _need_cuda("w_scale", w_scale, torch.float32)
+        if w_scale.numel() not in (1, N) or not w_scale.is_contiguous():
+            raise ValueError("w_scale must be a contiguous float32 tensor with 1 or N elements")
+    nb = 0 if bias is None else bias.numel()
+    if nb:
+        _need_cuda("bias", bias, out_dtype)
+        if nb != N or not bias.is_contiguous():
+            raise ValueError("bias must be contiguous with N elements, in the output dtype")
+    return M, N, K, 0 if w_scale is None else w_scale.numel(), nb
+
+
+def _out_matrix(M: int, N: int, dtype: torch.dtype, device) -> torch.Tensor:
+    """[M, N] with rows at a multiple of 16 bytes (contiguous when N allows)."""
+    per = 16 // dtype.itemsize
+    return torch.empty(M, -(-N // per) * per, dtype=dtype, device=device)[:, :N]
+
+
+def gemm_fp4(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: torch.Tensor,
+             x_scale: torch.Tensor | None = None, w_scale: torch.Tensor | None = None,
+             bias: torch.Tensor | None = None, kind: str = "nvfp4", out: torch.Tensor | None = None,
+             out_dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
+    """out = cast(((acc * x_scale[:, None]) * w_scale) + bias), acc the product of the 4-bit matrices
+    x [M, K] and w [N, K] (codes times block scales) accumulated in fp32.
+
+    x, w: codes, uint8 [., K / 2]; x_scale float32 [M] or None; w_scale [N], [1] or None; bias [N] in
+    the output dtype or None / empty; out [M, N] bf16 / fp16 / fp32 (allocated with rows at
+    a multiple of 16 bytes when not given)."""
+    code = _fp4_code(kind)
+    if out is not None:
+        out_dtype = out.dtype
+    if out_dtype not in OUT_CODE:
+        raise TypeError(f"out_dtype {out_dtype} is not one of {tuple(OUT_CODE)}")
+    M, N, K, nws, nb = _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype)
+    if out is None:
+        out = _out_matrix(M, N, out_dtype, x.device)
+    _need_cuda("out", out, out_dtype, 2)
+    if tuple(out.shape) != (M, N):
+        raise ValueError(f"out has shape {tuple(out.shape)}, expected {(M, N)}")
+    _one_device(x=x, w=w, x_sf=x_sf, w_sf=w_sf, x_scale=x_scale, w_scale=w_scale, bias=bias if nb else None, out=out)
+    with _on(x.device):
+        rc = _lib.load().t8g_gemm_fp4(
+            _ptr(x), _ptr(x_sf), _ptr(x_scale), _ptr(w), _ptr(w_sf), _ptr(w_scale), nws, _ptr(bias) if nb else None, nb,
+            _ptr(out), OUT_CODE[out_dtype], M, N, K, _pitch(x, 16), _pitch(w, 16), _pitch(out, 16 // out_dtype.itemsize),
+            code, _stream_handle(x.device, stream))
+    _lib.check(rc)
+    return out
+
+
+def gemm_fp4_gated(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: torch.Tensor,
+                   x_scale: torch.Tensor | None, w_scale: torch.Tensor | None, bias: torch.Tensor | None,
+                   res: torch.Tensor, gate: torch.Tensor, *, rows_per_gate: int | None = None,
+                   gate_index: torch.Tensor | None = None, kind: str = "nvfp4", out: torch.Tensor | None = None,
+                   stream=None) -> torch.Tensor:
+    """gemm_fp4 as the DiT block's gated residual: out = bf16(res + gate[g] * y), y the product in
+    float32 (one rounding, where gemm_gated keeps torch's three), g = gate_index[m] (trusted to be
+    rows of gate) or m // rows_per_gate; out may be res itself (in-place update)."""
+    code = _fp4_code(kind)
+    M, N, K, nws, nb = _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, torch.bfloat16)
+    _need_cuda("res", res, torch.bfloat16, 2)
+    if tuple(res.shape) != (M, N):
+        raise ValueError(f"res has shape {tuple(res.shape)}, expected {(M, N)}")
+    if gate.dim() == 1:
+        gate = gate.view(1, -1)
+    _need_cuda("gate", gate, torch.bfloat16, 2)
+    if gate.shape[1] != N or gate.shape[0] < 1:
+        raise ValueError(f"gate must be [n_gate, {N}], got {tuple(gate.shape)}")
+    if gate_index is not None:
+        _need_cuda("gate_index", gate_index, torch.int32, 1)
+        if gate_index.numel() != M or not gate_index.is_contiguous():
+            raise ValueError("gate_index must be a contiguous int32 tensor with M elements")
+        rpg = 0
+    else:
+        if rows_per_gate is None:
+            if M % gate.shape[0]:
+                raise ValueError(f"{M} rows do not split evenly over {gate.shape[0]} gate rows; pass gate_index")
+            rows_per_gate = max(1, M // gate.shape[0])
+        rpg = int(rows_per_gate)
+        if rpg < 1 or (M and (M - 1) // rpg >= gate.shape[0]):
+            raise ValueError(f"rows_per_gate={rpg} maps rows past the {gate.shape[0]} gate rows")
+    if out is None:
+        out = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
+    _need_cuda("out", out, torch.bfloat16, 2)
+    if tuple(out.shape) != (M, N):
+        raise ValueError(f"out has shape {tuple(out.shape)}, expected {(M, N)}")
+    _one_device(x=x, w=w, x_sf=x_sf, w_sf=w_sf, x_scale=x_scale, w_scale=w_scale, bias=bias if nb else None, res=res,
+                gate=gate, gate_index=gate_index, out=out)
+    with _on(x.device):
+        rc = _lib.load().t8g_gemm_fp4_gated(
+            _ptr(x), _ptr(x_sf), _ptr(x_scale), _ptr(w), _ptr(w_sf), _ptr(w_scale), nws, _ptr(bias) if nb else None, nb,
+            _ptr(res), _pitch(res, 8), _ptr(gate), _pitch(gate, 8), _ptr(gate_index), rpg, _ptr(out), M, N, K,
+            _pitch(x, 16), _pitch(w, 16), _pitch(out, 8), code, _stream_handle(x.device, stream))
+    _lib.check(rc)
+    return out
+
+
 def device_status(device=None, stream=None) -> int:
     """Synchronise and read/clear the device status word (0 = no wait ran out)."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)

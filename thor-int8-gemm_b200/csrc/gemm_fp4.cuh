@@ -278,5 +278,347 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 }
 
 
+// ---------------------------------------------------------------- 2-SM kernel
+// The 8-bit pair kernel's scheme (gemm.cuh): a cluster of two CTAs computes 256 x 256 tiles with
+// cta_group::2 MMAs, persistent over tiles.  What differs is the room in TMEM: two 256-column
+// accumulators would leave no columns for the scales.  The accumulators therefore overlap by kOver
+// columns,
+//     [0, 256)   [256 - kOver, 512 - kOver)   scales [512 - kOver, 512)
+// and a tile's epilogue reads the shared columns first and then reports them free, so that the next tile's
+// MMAs wait for one chunk of the epilogue, not for all of it.  (Tiles of 192 columns would need no
+// overlap, but feed the tensor cores 14 % more operand bytes per product.)
+// A CTA needs its own 128 rows' scales of A but those of all 256 rows of W: both CTAs load them.
+template <bool MX, int OUT>
+struct PairCfg {
+  static constexpr int kTiles = stage_tiles(MX);
+  static constexpr int kABytes = 128 * BK;
+  static constexpr int kBBytes = 128 * BK;
+  static constexpr int kSfaBytes = kTiles * kScaleTile;
+  static constexpr int kSfbBytes = 2 * kTiles * kScaleTile;
+  static constexpr int kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;
+  static constexpr int kStages = (MX && OUT != kOutGated) ? 5 : 4;
+  static constexpr int kOver = MX ? 32 : 64;             // >= 12 kTiles scale columns
+  static constexpr int kEpiBytes = OUT == kOutGated ? 16 : 4096;
+  static constexpr int kResBytes = OUT == kOutGated ? 4 * 4096 : 16;
+  struct Smem {
+    uint8_t a[kStages][kABytes];
+    uint8_t b[kStages][kBBytes];
+    alignas(1024) uint8_t epi[gemm::EPI_WARPS][2][kEpiBytes];
+    alignas(1024) uint8_t res[gemm::EPI_WARPS][kResBytes];
+    uint8_t gate[gemm::EPI_WARPS][OUT == kOutGated ? 512 : 16];
+    alignas(128) uint8_t sfa[kStages][kSfaBytes];
+    alignas(128) uint8_t sfb[kStages][kSfbBytes];
+    gemm::TileParams params[2];
+    uint64_t full[kStages];
+    uint64_t empty[kStages];
+    uint64_t tmem_full[2];
+    uint64_t shared_free;
+    uint64_t drain;
+    uint32_t tmem_base;
+  };
+  static constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+  static_assert(12 * kTiles <= kOver, "the scales fit the columns between the accumulators");
+};
+
+// ws (1 without weight scales) and bias of the tile's columns; 2-byte outputs take the bias as packed
+// pairs of the output type.
+template <int OUT>
+__device__ __forceinline__ void stage_params(const Args& args, int n_tile0, int e, gemm::TileParams& tp) {
+  for (int j = e; j < gemm::BN; j += 128) {
+    const int n = n_tile0 + j;
+    const bool in = n < args.N;
+    tp.ws[j] = args.ws == nullptr ? 1.f : in ? __ldg(args.ws + (args.ws_stride ? n : 0)) : 0.f;
+    tp.bias[j] = (in && args.bias) ? OutTraits<OUT>::to_f32(args.bias, n) : 0.f;
+  }
+  if constexpr (OUT != kOutF32) {
+    const uint16_t* b16 = static_cast<const uint16_t*>(args.bias);
+    const int n = n_tile0 + 2 * e;
+    const uint32_t lo = (args.bias && n < args.N) ? b16[n] : 0u;
+    const uint32_t hi = (args.bias && n + 1 < args.N) ? b16[n + 1] : 0u;
+    tp.bias2[e] = lo | (hi << 16);
+  }
+}
+
+// Epilogue of a warp's 32 x 256 slice of a tile.  `high_first`: the columns shared with the other
+// accumulator are the last kOver (else the first); they are read first and `shared_bar` (the
+// leader's, a cluster address) is then told.
+template <bool MX, int OUT>
+__device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMap* tm_out,
+                                              typename PairCfg<MX, OUT>::Smem& s, int ew, int& ebuf,
+                                              const gemm::GatedSlice& gs, uint32_t t_row, int row0, int n_tile0,
+                                              int lane, uint64_t pol_out, float xs_r, const gemm::TileParams& tp,
+                                              bool high_first, uint32_t shared_bar) {
+  constexpr int kCols = OUT == kOutF32 ? 32 : 64;
+  constexpr int kChunks = gemm::BN / kCols;
+  constexpr int kFirst = (PairCfg<MX, OUT>::kOver + kCols - 1) / kCols;   // chunks that hold the shared columns
+  const bool has_bias = args.bias != nullptr;
+  const float2 xs2 = make_float2(xs_r, xs_r);
+  const int tile_cols = min(gemm::BN, args.N - n_tile0);
+  if constexpr (OUT == kOutGated) {
+    cp_async_wait_all();
+    __syncwarp();
+  }
+  uint32_t r[kCols / 32][32];
+  auto load = [&](int i) {
+    const int c = high_first ? kChunks - 1 - i : i;
+#pragma unroll
+    for (int h = 0; h < kCols / 32; ++h) tmem_ld_32x32b_x32(t_row + static_cast<uint32_t>(c * kCols + 32 * h), r[h]);
+  };
+  load(0);
+#pragma unroll 1
+  for (int i = 0; i < kChunks; ++i) {
+    const int c = high_first ? kChunks - 1 - i : i;
+#pragma unroll
+    for (int h = 0; h < kCols / 32; ++h) tmem_ld_wait_regs(r[h]);
+    float v[kCols];
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) v[j] = __uint_as_float(r[j / 32][j % 32]);
+    if (i + 1 < kChunks) load(i + 1);
+    if (i == kFirst - 1) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(shared_bar);
+    }
+    if (c * kCols >= tile_cols) continue;
+    if constexpr (OUT == kOutF32) {
+      const float4* wq = reinterpret_cast<const float4*>(tp.ws + c * kCols);
+      const float4* bq = reinterpret_cast<const float4*>(tp.bias + c * kCols);
+      if (lane == 0) bulk_wait_group_read<1>();   // the staging buffer's last store has read it
+      __syncwarp();
+      uint8_t* buf = s.epi[ew][ebuf];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float4 w4 = wq[q], b4 = bq[q];
+        float4 o;
+        o.x = __fmul_rn(__fmul_rn(v[4 * q + 0], xs_r), w4.x);
+        o.y = __fmul_rn(__fmul_rn(v[4 * q + 1], xs_r), w4.y);
+        o.z = __fmul_rn(__fmul_rn(v[4 * q + 2], xs_r), w4.z);
+        o.w = __fmul_rn(__fmul_rn(v[4 * q + 3], xs_r), w4.w);
+        if (has_bias) o = make_float4(__fadd_rn(o.x, b4.x), __fadd_rn(o.y, b4.y), __fadd_rn(o.z, b4.z), __fadd_rn(o.w, b4.w));
+        *reinterpret_cast<float4*>(buf + lane * 128 + ((q ^ (lane & 7)) * 16)) = o;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(tm_out, buf, n_tile0 + c * kCols, row0, pol_out);
+        bulk_commit_group();
+      }
+      ebuf ^= 1;
+    } else if constexpr (OUT == kOutGated) {
+      const float4* wq = reinterpret_cast<const float4*>(tp.ws + c * kCols);
+      const uint4* bq2 = reinterpret_cast<const uint4*>(tp.bias2 + c * kCols / 2);
+      uint8_t* slot = s.res[ew] + c * 4096;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float4 w0 = wq[2 * q], w1 = wq[2 * q + 1];
+        const float2 wp[4] = {make_float2(w0.x, w0.y), make_float2(w0.z, w0.w), make_float2(w1.x, w1.y),
+                              make_float2(w1.z, w1.w)};
+        const uint4 b4 = has_bias ? bq2[q] : make_uint4(0, 0, 0, 0);
+        const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w};
+        const int col = c * kCols + 8 * q;
+        uint4* cell = reinterpret_cast<uint4*>(slot + lane * 128 + ((q ^ (lane & 7)) * 16));
+        const uint4 r4 = *cell;
+        uint4 g4 = make_uint4(0, 0, 0, 0);
+        if (gs.shared_gate)
+          g4 = *reinterpret_cast<const uint4*>(s.gate[ew] + (c * 8 + q) * 16);
+        else if (gs.gate_row != nullptr && col < tile_cols)
+          g4 = __ldg(reinterpret_cast<const uint4*>(gs.gate_row + col));
+        const uint32_t rw[4] = {r4.x, r4.y, r4.z, r4.w};
+        const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w};
+        uint32_t o[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          float2 f = mul2_rn(mul2_rn(make_float2(v[8 * q + 2 * p], v[8 * q + 2 * p + 1]), xs2), wp[p]);
+          if (has_bias) f = add_f32_bf16x2(f, bw[p]);
+          o[p] = f2_to_bf2(fma2_rn(bf2_to_f2(gw[p]), f, bf2_to_f2(rw[p])));
+        }
+        *cell = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_2d(tm_out, slot, n_tile0 + c * kCols, row0, pol_out);
+        bulk_commit_group();
+      }
+    } else {
+      uint32_t packed[32];
+      gemm::dequant_pack64<OUT>(tp, c, v, xs2, has_bias, packed);
+      gemm::store_chunk64<4096>(tm_out, s.epi[ew], ebuf, lane, packed, n_tile0 + c * kCols, row0, pol_out);
+    }
+  }
+}
+
+template <bool MX, int OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+    gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                         const __grid_constant__ CUtensorMap tm_sfa, const __grid_constant__ CUtensorMap tm_sfb,
+                         const __grid_constant__ CUtensorMap tm_out, const Args args) {
+  extern __shared__ uint8_t smem_raw[];
+  using C = PairCfg<MX, OUT>;
+  using gemm::BN;
+  using gemm::P_BM;
+  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+  typename C::Smem& s = *reinterpret_cast<typename C::Smem*>(smem_raw + pad);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const int pair = static_cast<int>(blockIdx.x >> 1);
+  const int npairs = static_cast<int>(gridDim.x >> 1);
+  const int tiles_n = (args.N + BN - 1) / BN;
+  const int num_tiles = (args.M + P_BM - 1) / P_BM * tiles_n;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    mbar_init(&s.tmem_full[0], 1);
+    mbar_init(&s.tmem_full[1], 1);
+    mbar_init(&s.shared_free, 2 * gemm::EPI_WARPS);
+    mbar_init(&s.drain, 1);
+    fence_mbarrier_init();
+    prefetch_tensormap(&tm_a);
+    prefetch_tensormap(&tm_b);
+    prefetch_tensormap(&tm_sfa);
+    prefetch_tensormap(&tm_sfb);
+    prefetch_tensormap(&tm_out);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&s.tmem_base, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();   // both CTAs' barriers initialised before any cross-CTA signal
+  tc_fence_after();
+  const uint32_t tmem_base = s.tmem_base;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer (both CTAs)
+    if (lane == 0) {
+      const uint64_t pol_a = policy_evict_normal();
+      const uint64_t pol_b = policy_evict_last();
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < num_tiles; tile += npairs) {
+        const int tm = tile / tiles_n;
+        const int tn = tile - tm * tiles_n;
+        for (int kb = 0; kb < args.kstages; ++kb) {
+          if (!mbar_wait(&s.empty[stage], phase ^ 1u, kStatusTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_arrive_expect_tx(&s.full[stage], 2 * C::kStageBytes);
+          const uint32_t bar = mapa_shared(smem_u32(&s.full[stage]), 0);
+          tma_load_2d_pair(s.a[stage], &tm_a, bar, kb * BK, tm * P_BM + rank * 128, pol_a);
+          tma_load_2d_pair(s.b[stage], &tm_b, bar, kb * BK, tn * BN + rank * 128, pol_b);
+          tma_load_2d_pair(s.sfa[stage], &tm_sfa, bar, kb * (C::kSfaBytes / 8), tm * 2 + rank, pol_a);
+          tma_load_2d_pair(s.sfb[stage], &tm_sfb, bar, kb * (C::kSfaBytes / 8), tn * 2, pol_b);
+          ++issued;
+          if (++stage == C::kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // the leader sees every copy of the pair land on its `full` barriers
+      if (rank == 0) {
+        for (int i = 0; i < C::kStages && i < issued; ++i) {
+          const int n = issued - 1 - i;
+          if (!mbar_wait(&s.full[n % C::kStages], static_cast<uint32_t>((n / C::kStages) & 1), kStatusTimeoutDrain)) break;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader only)
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = make_idesc_fp4(MX, P_BM, BN);
+      const uint32_t empty0[2] = {mapa_shared(smem_u32(&s.empty[0]), 0), mapa_shared(smem_u32(&s.empty[0]), 1)};
+      const uint32_t tfull0[2] = {mapa_shared(smem_u32(&s.tmem_full[0]), 0), mapa_shared(smem_u32(&s.tmem_full[0]), 1)};
+      const uint32_t sa_t = tmem_base + 512u - C::kOver;
+      const uint32_t sb_t = sa_t + 4u * C::kTiles;
+      int stage = 0, local = 0;
+      uint32_t phase = 0;
+      bool ok = true, any = false;
+      for (int tile = pair; ok && tile < num_tiles; tile += npairs, ++local) {
+        // the shared columns of the tile before; its own accumulator's other columns were read
+        // before that tile's epilogue began
+        if (local > 0 && !mbar_wait(&s.shared_free, static_cast<uint32_t>(local - 1) & 1u, kStatusTimeoutMma)) break;
+        tc_fence_after();
+        const int acc = local & 1;
+        const uint32_t d_tmem = tmem_base + (acc ? 256u - C::kOver : 0u);
+        for (int kb = 0; kb < args.kstages; ++kb) {
+          if (!mbar_wait(&s.full[stage], phase, kStatusTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          stage_mmas<MX, true, 2>(d_tmem, smem_u32(s.a[stage]), smem_u32(s.b[stage]), smem_u32(s.sfa[stage]),
+                                  smem_u32(s.sfb[stage]), sa_t, sb_t, 0u, idesc,
+                                  kb == args.kstages - 1 ? args.last_steps : kStageK / kMmaK, kb == 0);
+          tc_commit_pair(empty0[0] + 8u * static_cast<uint32_t>(stage));
+          tc_commit_pair(empty0[1] + 8u * static_cast<uint32_t>(stage));
+          any = true;
+          if (++stage == C::kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        tc_commit_pair(tfull0[0] + 8u * static_cast<uint32_t>(acc));
+        tc_commit_pair(tfull0[1] + 8u * static_cast<uint32_t>(acc));
+      }
+      if (any) {
+        tc_commit_pair(mapa_shared(smem_u32(&s.drain), 0));
+        mbar_wait(&s.drain, 0, kStatusTimeoutDrain);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue (both CTAs)
+    const int ew = warp - 2;
+    const int quarter = warp & 3;
+    const int e = threadIdx.x - 64;
+    const uint64_t pol_out = policy_evict_first();
+    const uint32_t shared_bar = mapa_shared(smem_u32(&s.shared_free), 0);
+    int local = 0, ebuf = 0;
+    for (int tile = pair; tile < num_tiles; tile += npairs, ++local) {
+      const int tm = tile / tiles_n;
+      const int tn = tile - tm * tiles_n;
+      const int acc = local & 1;
+      const int row0 = tm * P_BM + rank * 128 + quarter * 32;
+      stage_params<OUT>(args, tn * BN, e, s.params[acc]);
+      const float xs_r = (row0 + lane < args.M && args.xs) ? __ldg(args.xs + row0 + lane) : 1.f;
+      gemm::GatedSlice gs{};
+      if constexpr (OUT == kOutGated) {
+        if (row0 < args.M) gs = gemm::gated_prefetch(args, s.res[ew], s.gate[ew], row0, tn * BN, lane);
+      }
+      const bool ok = mbar_wait(&s.tmem_full[acc], static_cast<uint32_t>((local >> 1) & 1), kStatusTimeoutEpilogue);
+      // all four warps staged the parameters; they leave together if any wait ran out
+      if (named_bar_any(1, 128, !ok)) break;
+      tc_fence_after();
+      if (row0 < args.M) {
+        const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (acc ? 256u - C::kOver : 0u);
+        epilogue_pair<MX, OUT>(args, &tm_out, s, ew, ebuf, gs, t_row, row0, tn * BN, lane, pol_out, xs_r, s.params[acc],
+                               acc == 0, shared_bar);
+      } else if (lane == 0) {
+        mbar_arrive_cluster(shared_bar);
+      }
+    }
+    if constexpr (OUT == kOutGated) cp_async_wait_all();   // a residual copy left by a wait that gave up
+    if (lane == 0) bulk_wait_group_all();
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();   // the pair's MMAs, copies and cross-CTA signals are all done
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
 }  // namespace gemm4
 }  // namespace t8g

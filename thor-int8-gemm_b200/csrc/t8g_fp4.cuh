@@ -90,7 +90,50 @@ int launch_gemm_fp4_small(const Fp4Gemm& p, const t8g::gemm4::Args& args, int sp
 }
 
 template <bool MX, int OUT>
+int launch_gemm_fp4_pair(const Fp4Gemm& p, const t8g::gemm4::Args& args, int dev, int sms, cudaStream_t st) {
+  using namespace t8g::gemm4;
+  using C = PairCfg<MX, OUT>;
+  static std::atomic<bool> attr_done[kMaxDevices] = {};
+  auto kern = gemm_fp4_pair_kernel<MX, OUT>;
+  int rc = ensure_smem_attr(kern, dev, C::kSmemBytes, attr_done);
+  if (rc) return rc;
+  const int64_t words = fp4_words(p.K, p.kind);
+  const uint32_t sf_box = C::kSfaBytes / 8;
+  constexpr int esz = OutTraits<OUT>::kBytes;
+  CUtensorMap ta, tb, tsa, tsb, to;
+  if ((rc = encode_2d(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.x, p.K / 2, p.M, p.ld_x, BK, 128, CU_TENSOR_MAP_SWIZZLE_128B)))
+    return rc;
+  if ((rc = encode_2d(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.K / 2, p.N, p.ld_w, BK, 128, CU_TENSOR_MAP_SWIZZLE_128B)))
+    return rc;
+  if ((rc = encode_2d(&tsa, CU_TENSOR_MAP_DATA_TYPE_INT64, p.x_sf, words * 64, (p.M + 127) / 128, words * 512, sf_box, 1,
+                      CU_TENSOR_MAP_SWIZZLE_NONE)))
+    return rc;
+  if ((rc = encode_2d(&tsb, CU_TENSOR_MAP_DATA_TYPE_INT64, p.w_sf, words * 64, (p.N + 127) / 128, words * 512, sf_box, 2,
+                      CU_TENSOR_MAP_SWIZZLE_NONE)))
+    return rc;
+  const CUtensorMapDataType out_dt = OUT == kOutF32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : OUT == kOutF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  // 32 rows of 128 bytes: 64 two-byte or 32 four-byte columns
+  if ((rc = encode_2d(&to, out_dt, args.out, p.N, p.M, args.ld_out * esz, 128 / esz, 32, CU_TENSOR_MAP_SWIZZLE_128B)))
+    return rc;
+  const int64_t tiles = ((p.M + 255) / 256) * ((p.N + 255) / 256);
+  if (tiles >= (int64_t(1) << 31)) return fail(T8G_ERR_UNSUPPORTED, "gemm_fp4: too many tiles");
+  const int64_t pairs = std::min<int64_t>(tiles, sms / 2);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs), 1, 1);
+  cfg.blockDim = dim3(NUM_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.stream = st;
+  cfg.attrs = nullptr;   // the kernel declares its cluster shape (2, 1, 1)
+  cfg.numAttrs = 0;
+  T8G_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, ta, tb, tsa, tsb, to, args), "gemm_fp4 pair launch");
+  return T8G_OK;
+}
+
+template <bool MX, int OUT>
 int launch_gemm_fp4(const Fp4Gemm& p, const t8g::gemm4::Args& args, int dev, int sms, cudaStream_t st) {
+  if (((p.M + 255) / 256) * ((p.N + 255) / 256) * 4 >= sms) return launch_gemm_fp4_pair<MX, OUT>(p, args, dev, sms, st);
   const int64_t tm = (p.M + 127) / 128;
   const bool narrow = tm * ((p.N + 127) / 128) < sms;
   const int64_t tiles = tm * ((p.N + (narrow ? 63 : 127)) / (narrow ? 64 : 128));

@@ -45,33 +45,47 @@ struct Args : gemm::Args {
   int64_t ld_out;
 };
 
-// MMAs of one stage: copy its scales to TMEM, then `steps` K = 64 products.  `sa_t` / `sb_t`:
-// TMEM columns of A's scales (4 per tile) and B's (4 * B_GROUPS per tile); `sb_off`: first
-// column of this tile's rows within B's scale word columns.
-template <bool MX, bool PAIR, int B_GROUPS>
-__device__ __forceinline__ void stage_mmas(uint32_t d_tmem, uint32_t a0, uint32_t b0, uint32_t sfa, uint32_t sfb,
-                                           uint32_t sa_t, uint32_t sb_t, uint32_t sb_off, uint32_t idesc, int steps,
-                                           bool first) {
+// Shared-memory descriptors of stage 0; a stage further on adds its bytes / 16 to the address field
+// (14 bits, which hold any shared-memory address / 16, so the sum never leaves it).
+struct StageDescs {
+  uint64_t a, b, sfa, sfb;
+};
+
+// MMAs of one stage, issued by one elected lane: copy its scales to TMEM, then `steps` K = 64
+// products.  `sa_t` / `sb_t`: TMEM columns of A's scales (4 per tile) and B's (4 * B_GROUPS per
+// tile), B's moved by `sb_off` to this output tile's rows.
+template <bool MX, bool PAIR, int B_GROUPS, int STEPS>
+__device__ __forceinline__ void stage_mmas_n(uint32_t d_tmem, const StageDescs& d, uint32_t sa_t, uint32_t sb_t,
+                                             uint32_t sb_off, uint32_t idesc, uint32_t accumulate) {
   constexpr int kTiles = stage_tiles(MX);
-  const int tiles = MX ? (steps + 1) >> 1 : steps;
+  constexpr int kUsed = MX ? (STEPS + 1) / 2 : STEPS;
 #pragma unroll
-  for (int t = 0; t < kTiles; ++t) {
-    if (t < tiles) {
-      tmem_cp_scales<PAIR>(sa_t + 4u * t, smem_desc_scales(sfa + t * kScaleTile));
+  for (int t = 0; t < kUsed; ++t) {
+    tmem_cp_scales<PAIR>(sa_t + 4u * t, d.sfa + t * (kScaleTile / 16));
 #pragma unroll
-      for (int g = 0; g < B_GROUPS; ++g)
-        tmem_cp_scales<PAIR>(sb_t + 4u * (B_GROUPS * t + g), smem_desc_scales(sfb + (g * kTiles + t) * kScaleTile));
-    }
+    for (int g = 0; g < B_GROUPS; ++g)
+      tmem_cp_scales<PAIR>(sb_t + 4u * (B_GROUPS * t + g), d.sfb + (g * kTiles + t) * (kScaleTile / 16));
   }
 #pragma unroll
-  for (int k = 0; k < kStageK / kMmaK; ++k) {
-    if (k < steps) {
-      const uint32_t t = MX ? k >> 1 : k;
-      const uint32_t id = MX ? static_cast<uint32_t>(k & 1) * ((2u << 29) | (2u << 4)) : 0u;
-      mma_fp4<MX, PAIR>(d_tmem, smem_desc_k_sw128(a0 + k * 32), smem_desc_k_sw128(b0 + k * 32), idesc | id,
-                        sa_t + 4u * t, sb_t + 4u * B_GROUPS * t + sb_off, (first && k == 0) ? 0u : 1u);
-    }
+  for (int k = 0; k < STEPS; ++k) {
+    const uint32_t t = MX ? k >> 1 : k;
+    const uint32_t id = MX ? static_cast<uint32_t>(k & 1) * ((2u << 29) | (2u << 4)) : 0u;
+    mma_fp4<MX, PAIR>(d_tmem, d.a + 2 * k, d.b + 2 * k, idesc | id, sa_t + 4u * t, sb_t + 4u * B_GROUPS * t + sb_off,
+                      k == 0 ? accumulate : 1u);
   }
+}
+
+template <bool MX, bool PAIR, int B_GROUPS>
+__device__ __forceinline__ void stage_mmas(uint32_t d_tmem, const StageDescs& d, uint32_t sa_t, uint32_t sb_t,
+                                           uint32_t sb_off, uint32_t idesc, int steps, uint32_t accumulate) {
+  if (steps == 4)
+    stage_mmas_n<MX, PAIR, B_GROUPS, 4>(d_tmem, d, sa_t, sb_t, sb_off, idesc, accumulate);
+  else if (steps == 3)
+    stage_mmas_n<MX, PAIR, B_GROUPS, 3>(d_tmem, d, sa_t, sb_t, sb_off, idesc, accumulate);
+  else if (steps == 2)
+    stage_mmas_n<MX, PAIR, B_GROUPS, 2>(d_tmem, d, sa_t, sb_t, sb_off, idesc, accumulate);
+  else
+    stage_mmas_n<MX, PAIR, B_GROUPS, 1>(d_tmem, d, sa_t, sb_t, sb_off, idesc, accumulate);
 }
 
 // ---------------------------------------------------------------- epilogue arithmetic
@@ -189,27 +203,33 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = make_idesc_fp4(MX, BM, TBN);
-      const uint32_t sb_off = static_cast<uint32_t>(tn * TBN % BM / 32);
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&s.full[stage], phase, kStatusTimeoutMma)) break;
-        tc_fence_after();
+    constexpr uint32_t idesc = make_idesc_fp4(MX, BM, TBN);
+    const uint32_t sb_off = static_cast<uint32_t>(tn * TBN % BM / 32);
+    const StageDescs d0 = {smem_desc_k_sw128(smem_u32(s.a[0])), smem_desc_k_sw128(smem_u32(s.b[0])),
+                           smem_desc_scales(smem_u32(s.sfa[0])), smem_desc_scales(smem_u32(s.sfb[0]))};
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait_warp(&s.full[stage], phase, kStatusTimeoutMma)) break;
+      tc_fence_after();
+      if (elect_one()) {
         const uint32_t sa_t = tmem_base + TBN + static_cast<uint32_t>(kb & 1) * C::kSfCols;
-        stage_mmas<MX, false, 1>(tmem_base, smem_u32(s.a[stage]), smem_u32(s.b[stage]), smem_u32(s.sfa[stage]),
-                                 smem_u32(s.sfb[stage]), sa_t, sa_t + 4u * C::kTiles, sb_off, idesc,
-                                 kb == args.kstages - 1 ? args.last_steps : kStageK / kMmaK, kb == kb0);
+        const StageDescs d = {d0.a + stage * (C::kABytes / 16), d0.b + stage * (C::kBBytes / 16),
+                              d0.sfa + stage * (C::kSfBytes / 16), d0.sfb + stage * (C::kSfBytes / 16)};
+        stage_mmas<MX, false, 1>(tmem_base, d, sa_t, sa_t + 4u * C::kTiles, sb_off, idesc,
+                                 kb == args.kstages - 1 ? args.last_steps : kStageK / kMmaK, kb != kb0);
         tc_commit(&s.empty[stage]);
-        if (++stage == C::kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        if (kb == kb1 - 1) tc_commit(&s.done);
       }
-      tc_commit(&s.done);   // also when a wait gave up: completes once the issued MMAs have
-      mbar_wait(&s.done, 0, kStatusTimeoutDrain);
+      __syncwarp();
+      if (++stage == C::kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
     }
+    // every MMA (and its shared-memory reads) completes before teardown; a wait that gave up leaves
+    // `done` to the waits' own limits
+    mbar_wait_warp(&s.done, 0, kStatusTimeoutDrain);
   } else {
     have = mbar_wait(&s.done, 0, kStatusTimeoutEpilogue);
     tc_fence_after();
@@ -533,46 +553,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader only)
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr uint32_t idesc = make_idesc_fp4(MX, P_BM, BN);
       const uint32_t empty0[2] = {mapa_shared(smem_u32(&s.empty[0]), 0), mapa_shared(smem_u32(&s.empty[0]), 1)};
       const uint32_t tfull0[2] = {mapa_shared(smem_u32(&s.tmem_full[0]), 0), mapa_shared(smem_u32(&s.tmem_full[0]), 1)};
       const uint32_t sa_t = tmem_base + 512u - C::kOver;
       const uint32_t sb_t = sa_t + 4u * C::kTiles;
+      const StageDescs d0 = {smem_desc_k_sw128(smem_u32(s.a[0])), smem_desc_k_sw128(smem_u32(s.b[0])),
+                             smem_desc_scales(smem_u32(s.sfa[0])), smem_desc_scales(smem_u32(s.sfb[0]))};
       int stage = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true, any = false;
       for (int tile = pair; ok && tile < num_tiles; tile += npairs, ++local) {
         // the shared columns of the tile before; its own accumulator's other columns were read
         // before that tile's epilogue began
-        if (local > 0 && !mbar_wait(&s.shared_free, static_cast<uint32_t>(local - 1) & 1u, kStatusTimeoutMma)) break;
+        if (local > 0 && !mbar_wait_warp(&s.shared_free, static_cast<uint32_t>(local - 1) & 1u, kStatusTimeoutMma)) break;
         tc_fence_after();
         const int acc = local & 1;
         const uint32_t d_tmem = tmem_base + (acc ? 256u - C::kOver : 0u);
         for (int kb = 0; kb < args.kstages; ++kb) {
-          if (!mbar_wait(&s.full[stage], phase, kStatusTimeoutMma)) {
+          if (!mbar_wait_warp(&s.full[stage], phase, kStatusTimeoutMma)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          stage_mmas<MX, true, 2>(d_tmem, smem_u32(s.a[stage]), smem_u32(s.b[stage]), smem_u32(s.sfa[stage]),
-                                  smem_u32(s.sfb[stage]), sa_t, sb_t, 0u, idesc,
-                                  kb == args.kstages - 1 ? args.last_steps : kStageK / kMmaK, kb == 0);
-          tc_commit_pair(empty0[0] + 8u * static_cast<uint32_t>(stage));
-          tc_commit_pair(empty0[1] + 8u * static_cast<uint32_t>(stage));
+          if (elect_one()) {
+            const StageDescs d = {d0.a + stage * (C::kABytes / 16), d0.b + stage * (C::kBBytes / 16),
+                                  d0.sfa + stage * (C::kSfaBytes / 16), d0.sfb + stage * (C::kSfbBytes / 16)};
+            stage_mmas<MX, true, 2>(d_tmem, d, sa_t, sb_t, 0u, idesc,
+                                    kb == args.kstages - 1 ? args.last_steps : kStageK / kMmaK, kb != 0);
+            tc_commit_pair(empty0[0] + 8u * static_cast<uint32_t>(stage));
+            tc_commit_pair(empty0[1] + 8u * static_cast<uint32_t>(stage));
+            if (kb == args.kstages - 1) {
+              tc_commit_pair(tfull0[0] + 8u * static_cast<uint32_t>(acc));
+              tc_commit_pair(tfull0[1] + 8u * static_cast<uint32_t>(acc));
+            }
+          }
+          __syncwarp();
           any = true;
           if (++stage == C::kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (!ok) break;
-        tc_commit_pair(tfull0[0] + 8u * static_cast<uint32_t>(acc));
-        tc_commit_pair(tfull0[1] + 8u * static_cast<uint32_t>(acc));
       }
       if (any) {
-        tc_commit_pair(mapa_shared(smem_u32(&s.drain), 0));
-        mbar_wait(&s.drain, 0, kStatusTimeoutDrain);
+        if (elect_one()) tc_commit_pair(mapa_shared(smem_u32(&s.drain), 0));
+        __syncwarp();
+        mbar_wait_warp(&s.drain, 0, kStatusTimeoutDrain);
       }
     }
   } else {

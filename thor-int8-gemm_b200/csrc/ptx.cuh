@@ -459,4 +459,24 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
+// True in one lane of a fully active warp.  A loop that the whole warp runs, with only the
+// issue of tcgen05 instructions inside `if (elect_one())`, keeps their operands in uniform
+// registers; issued from a loop that only lane 0 runs, every operand is moved there first.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n"
+      "  .reg .pred p;\n"
+      "  elect.sync _|p, 0xffffffff;\n"
+      "  selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(r));
+  return r != 0;
+}
+
+// mbar_wait by a whole warp that stays together: false in every lane if any lane's wait ran out.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int code) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, code));
+}
+
 }  // namespace t8g

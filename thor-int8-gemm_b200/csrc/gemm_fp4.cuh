@@ -308,6 +308,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 // MMAs wait for one chunk of the epilogue, not for all of it.  (Tiles of 192 columns would need no
 // overlap, but feed the tensor cores 14 % more operand bytes per product.)
 // A CTA needs its own 128 rows' scales of A but those of all 256 rows of W: both CTAs load them.
+//
+// Eight epilogue warps (four would take 4.6 us a tile, more than the 3.2 us that its MMAs take at K = 3072):
+// warp 2 + 4 h + i reads the 32 lanes 32 ((2 + i) % 4) .. of columns [128 h, 128 h + 128).
+constexpr int kEpiWarps = 8;
+constexpr int kPairThreads = 64 + 32 * kEpiWarps;
+constexpr int kHalfCols = gemm::BN / 2;
+
 template <bool MX, int OUT>
 struct PairCfg {
   static constexpr int kTiles = stage_tiles(MX);
@@ -316,16 +323,14 @@ struct PairCfg {
   static constexpr int kSfaBytes = kTiles * kScaleTile;
   static constexpr int kSfbBytes = 2 * kTiles * kScaleTile;
   static constexpr int kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;
+  static constexpr int kEpiBufs = OUT == kOutGated ? 2 : 1;   // 4 KB pieces per warp (gated: its whole residual slice)
   static constexpr int kStages = (MX && OUT != kOutGated) ? 5 : 4;
   static constexpr int kOver = MX ? 32 : 64;             // >= 12 kTiles scale columns
-  static constexpr int kEpiBytes = OUT == kOutGated ? 16 : 4096;
-  static constexpr int kResBytes = OUT == kOutGated ? 4 * 4096 : 16;
   struct Smem {
     uint8_t a[kStages][kABytes];
     uint8_t b[kStages][kBBytes];
-    alignas(1024) uint8_t epi[gemm::EPI_WARPS][2][kEpiBytes];
-    alignas(1024) uint8_t res[gemm::EPI_WARPS][kResBytes];
-    uint8_t gate[gemm::EPI_WARPS][OUT == kOutGated ? 512 : 16];
+    alignas(1024) uint8_t epi[kEpiWarps][kEpiBufs][4096];
+    uint8_t gate[kEpiWarps][OUT == kOutGated ? 2 * kHalfCols : 16];
     alignas(128) uint8_t sfa[kStages][kSfaBytes];
     alignas(128) uint8_t sfb[kStages][kSfbBytes];
     gemm::TileParams params[2];
@@ -345,90 +350,106 @@ struct PairCfg {
 // pairs of the output type.
 template <int OUT>
 __device__ __forceinline__ void stage_params(const Args& args, int n_tile0, int e, gemm::TileParams& tp) {
-  for (int j = e; j < gemm::BN; j += 128) {
-    const int n = n_tile0 + j;
-    const bool in = n < args.N;
-    tp.ws[j] = args.ws == nullptr ? 1.f : in ? __ldg(args.ws + (args.ws_stride ? n : 0)) : 0.f;
-    tp.bias[j] = (in && args.bias) ? OutTraits<OUT>::to_f32(args.bias, n) : 0.f;
-  }
-  if constexpr (OUT != kOutF32) {
-    const uint16_t* b16 = static_cast<const uint16_t*>(args.bias);
-    const int n = n_tile0 + 2 * e;
-    const uint32_t lo = (args.bias && n < args.N) ? b16[n] : 0u;
-    const uint32_t hi = (args.bias && n + 1 < args.N) ? b16[n + 1] : 0u;
-    tp.bias2[e] = lo | (hi << 16);
+  static_assert(gemm::BN == 32 * kEpiWarps, "one column per epilogue thread");
+  const int n = n_tile0 + e;
+  const bool in = n < args.N;
+  tp.ws[e] = args.ws == nullptr ? 1.f : in ? __ldg(args.ws + (args.ws_stride ? n : 0)) : 0.f;
+  if constexpr (OUT == kOutF32) {
+    tp.bias[e] = (in && args.bias) ? static_cast<const float*>(args.bias)[n] : 0.f;
+  } else {
+    reinterpret_cast<uint16_t*>(tp.bias2)[e] = (in && args.bias) ? static_cast<const uint16_t*>(args.bias)[n] : 0;
   }
 }
 
-// Epilogue of a warp's 32 x 256 slice of a tile.  `high_first`: the columns shared with the other
-// accumulator are the last kOver (else the first); they are read first and `shared_bar` (the
-// leader's, a cluster address) is then told.
+// Gated form: the residual rows of a warp's 32 x 128 slice are copied into its staging pieces (the
+// layout of the stores: 16-byte piece q of row r at q ^ (r & 7)) while the tile's MMAs run, each
+// then replaced by the output and stored from there; a gate row that all 32 rows share is
+// copied beside them.
+struct GatedSlice {
+  const uint16_t* gate_row;   // this lane's gate row at the slice's first column (null: row >= M)
+  bool shared_gate;           // every valid row of the warp uses lane 0's gate row
+};
+__device__ __forceinline__ GatedSlice gated_prefetch(const Args& args, uint8_t (*rbuf)[4096], uint8_t* gbuf, int row0,
+                                                     int n0, int lane) {
+  GatedSlice g;
+  const int m = row0 + lane;
+  const int cols = args.N - n0;   // may be <= 0
+  const uint16_t* res_row = nullptr;
+  int64_t grow = -1;
+  if (m < args.M) {
+    res_row = static_cast<const uint16_t*>(args.res) + static_cast<int64_t>(m) * args.ld_res + n0;
+    grow = args.gate_index ? static_cast<int64_t>(__ldg(args.gate_index + m)) : m / args.rows_per_gate;
+  }
+  g.gate_row = m < args.M ? static_cast<const uint16_t*>(args.gate) + grow * args.ld_gate + n0 : nullptr;
+  const int64_t grow0 = __shfl_sync(0xffffffffu, grow, 0);
+  g.shared_gate = __all_sync(0xffffffffu, m >= args.M || grow == grow0);
+  if (lane == 0) bulk_wait_group_read<0>();   // the previous tile's stores have read the pieces
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < kHalfCols / 64; ++c) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int col = c * 64 + 8 * q;
+      const bool in = res_row != nullptr && col < cols;
+      cp_async_16(rbuf[c] + lane * 128 + ((q ^ (lane & 7)) * 16),
+                  in ? static_cast<const void*>(res_row + col) : gemm::rbuf_src_dummy(), in ? 16u : 0u);
+    }
+  }
+  if (g.shared_gate && lane < kHalfCols / 8) {
+    const uint16_t* g0 = static_cast<const uint16_t*>(args.gate) + grow0 * args.ld_gate + n0;
+    const bool in = 8 * lane < cols;
+    cp_async_16(gbuf + lane * 16, in ? static_cast<const void*>(g0 + 8 * lane) : gemm::rbuf_src_dummy(), in ? 16u : 0u);
+  }
+  cp_async_commit();
+  return g;
+}
+
+// Epilogue of a warp's 32 x 128 slice of a tile (columns n0 .. of the output, `half` of the tile).
+// `shared`: this half holds the columns that the other accumulator uses too, its last ones if half is
+// 1 and its first if it is 0; they are read first and `shared_bar` (the leader's, a cluster
+// address) is then told.
 template <bool MX, int OUT>
 __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMap* tm_out,
-                                              typename PairCfg<MX, OUT>::Smem& s, int ew, int& ebuf,
-                                              const gemm::GatedSlice& gs, uint32_t t_row, int row0, int n_tile0,
-                                              int lane, uint64_t pol_out, float xs_r, const gemm::TileParams& tp,
-                                              bool high_first, uint32_t shared_bar) {
+                                              typename PairCfg<MX, OUT>::Smem& s, int ew, int half,
+                                              const GatedSlice& gs, uint32_t t_row, int row0, int n0, int lane,
+                                              uint64_t pol_out, float xs_r, const gemm::TileParams& tp, bool shared,
+                                              uint32_t shared_bar) {
   constexpr int kCols = OUT == kOutF32 ? 32 : 64;
-  constexpr int kChunks = gemm::BN / kCols;
+  constexpr int kChunks = kHalfCols / kCols;
   constexpr int kFirst = (PairCfg<MX, OUT>::kOver + kCols - 1) / kCols;   // chunks that hold the shared columns
   const bool has_bias = args.bias != nullptr;
   const float2 xs2 = make_float2(xs_r, xs_r);
-  const int tile_cols = min(gemm::BN, args.N - n_tile0);
+  const int cols = args.N - n0;
   if constexpr (OUT == kOutGated) {
     cp_async_wait_all();
     __syncwarp();
   }
   uint32_t r[kCols / 32][32];
   auto load = [&](int i) {
-    const int c = high_first ? kChunks - 1 - i : i;
+    const int c = half ? kChunks - 1 - i : i;
 #pragma unroll
     for (int h = 0; h < kCols / 32; ++h) tmem_ld_32x32b_x32(t_row + static_cast<uint32_t>(c * kCols + 32 * h), r[h]);
   };
   load(0);
 #pragma unroll 1
   for (int i = 0; i < kChunks; ++i) {
-    const int c = high_first ? kChunks - 1 - i : i;
+    const int c = half ? kChunks - 1 - i : i;
 #pragma unroll
     for (int h = 0; h < kCols / 32; ++h) tmem_ld_wait_regs(r[h]);
     float v[kCols];
 #pragma unroll
     for (int j = 0; j < kCols; ++j) v[j] = __uint_as_float(r[j / 32][j % 32]);
-    if (i + 1 < kChunks) load(i + 1);
-    if (i == kFirst - 1) {
+    if (shared && i == kFirst - 1) {   // the next tile's MMAs wait for this
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(shared_bar);
     }
-    if (c * kCols >= tile_cols) continue;
-    if constexpr (OUT == kOutF32) {
-      const float4* wq = reinterpret_cast<const float4*>(tp.ws + c * kCols);
-      const float4* bq = reinterpret_cast<const float4*>(tp.bias + c * kCols);
-      if (lane == 0) bulk_wait_group_read<1>();   // the staging buffer's last store has read it
-      __syncwarp();
-      uint8_t* buf = s.epi[ew][ebuf];
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const float4 w4 = wq[q], b4 = bq[q];
-        float4 o;
-        o.x = __fmul_rn(__fmul_rn(v[4 * q + 0], xs_r), w4.x);
-        o.y = __fmul_rn(__fmul_rn(v[4 * q + 1], xs_r), w4.y);
-        o.z = __fmul_rn(__fmul_rn(v[4 * q + 2], xs_r), w4.z);
-        o.w = __fmul_rn(__fmul_rn(v[4 * q + 3], xs_r), w4.w);
-        if (has_bias) o = make_float4(__fadd_rn(o.x, b4.x), __fadd_rn(o.y, b4.y), __fadd_rn(o.z, b4.z), __fadd_rn(o.w, b4.w));
-        *reinterpret_cast<float4*>(buf + lane * 128 + ((q ^ (lane & 7)) * 16)) = o;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        tma_store_2d(tm_out, buf, n_tile0 + c * kCols, row0, pol_out);
-        bulk_commit_group();
-      }
-      ebuf ^= 1;
-    } else if constexpr (OUT == kOutGated) {
-      const float4* wq = reinterpret_cast<const float4*>(tp.ws + c * kCols);
-      const uint4* bq2 = reinterpret_cast<const uint4*>(tp.bias2 + c * kCols / 2);
-      uint8_t* slot = s.res[ew] + c * 4096;
+    if (i + 1 < kChunks) load(i + 1);
+    if (c * kCols >= cols) continue;
+    const float4* wq = reinterpret_cast<const float4*>(tp.ws + half * kHalfCols + c * kCols);
+    uint8_t* buf = s.epi[ew][OUT == kOutGated ? c : 0];
+    if constexpr (OUT == kOutGated) {
+      const uint4* bq2 = reinterpret_cast<const uint4*>(tp.bias2 + (half * kHalfCols + c * kCols) / 2);
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         const float4 w0 = wq[2 * q], w1 = wq[2 * q + 1];
@@ -437,12 +458,12 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
         const uint4 b4 = has_bias ? bq2[q] : make_uint4(0, 0, 0, 0);
         const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w};
         const int col = c * kCols + 8 * q;
-        uint4* cell = reinterpret_cast<uint4*>(slot + lane * 128 + ((q ^ (lane & 7)) * 16));
+        uint4* cell = reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) * 16));
         const uint4 r4 = *cell;
         uint4 g4 = make_uint4(0, 0, 0, 0);
         if (gs.shared_gate)
           g4 = *reinterpret_cast<const uint4*>(s.gate[ew] + (c * 8 + q) * 16);
-        else if (gs.gate_row != nullptr && col < tile_cols)
+        else if (gs.gate_row != nullptr && col < cols)
           g4 = __ldg(reinterpret_cast<const uint4*>(gs.gate_row + col));
         const uint32_t rw[4] = {r4.x, r4.y, r4.z, r4.w};
         const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w};
@@ -455,22 +476,53 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
         }
         *cell = make_uint4(o[0], o[1], o[2], o[3]);
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        tma_store_2d(tm_out, slot, n_tile0 + c * kCols, row0, pol_out);
-        bulk_commit_group();
-      }
     } else {
-      uint32_t packed[32];
-      gemm::dequant_pack64<OUT>(tp, c, v, xs2, has_bias, packed);
-      gemm::store_chunk64<4096>(tm_out, s.epi[ew], ebuf, lane, packed, n_tile0 + c * kCols, row0, pol_out);
+      const float4* bq = reinterpret_cast<const float4*>(tp.bias + half * kHalfCols + c * kCols);
+      const uint4* bq2 = reinterpret_cast<const uint4*>(tp.bias2 + (half * kHalfCols + c * kCols) / 2);
+      uint4 o[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        if constexpr (OUT == kOutF32) {
+          const float4 w4 = wq[q], b4 = bq[q];
+          float2 f0 = mul2_rn(mul2_rn(make_float2(v[4 * q], v[4 * q + 1]), xs2), make_float2(w4.x, w4.y));
+          float2 f1 = mul2_rn(mul2_rn(make_float2(v[4 * q + 2], v[4 * q + 3]), xs2), make_float2(w4.z, w4.w));
+          if (has_bias) {
+            f0 = make_float2(__fadd_rn(f0.x, b4.x), __fadd_rn(f0.y, b4.y));
+            f1 = make_float2(__fadd_rn(f1.x, b4.z), __fadd_rn(f1.y, b4.w));
+          }
+          o[q] = make_uint4(__float_as_uint(f0.x), __float_as_uint(f0.y), __float_as_uint(f1.x), __float_as_uint(f1.y));
+        } else {
+          const float4 w0 = wq[2 * q], w1 = wq[2 * q + 1];
+          const float2 wp[4] = {make_float2(w0.x, w0.y), make_float2(w0.z, w0.w), make_float2(w1.x, w1.y),
+                                make_float2(w1.z, w1.w)};
+          const uint4 b4 = has_bias ? bq2[q] : make_uint4(0, 0, 0, 0);
+          const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w};
+          uint32_t h[4];
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            float2 f = mul2_rn(mul2_rn(make_float2(v[8 * q + 2 * p], v[8 * q + 2 * p + 1]), xs2), wp[p]);
+            if (has_bias) f = OUT == kOutF16 ? add_f32_f16x2(f, bw[p]) : add_f32_bf16x2(f, bw[p]);
+            h[p] = OutTraits<OUT>::pack2(f.x, f.y);
+          }
+          o[q] = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+      }
+      if (lane == 0) bulk_wait_group_read<0>();   // the warp's previous store has read the piece
+      __syncwarp();
+#pragma unroll
+      for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) * 16)) = o[q];
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(tm_out, buf, n0 + c * kCols, row0, pol_out);
+      bulk_commit_group();
     }
   }
 }
 
 template <bool MX, int OUT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                          const __grid_constant__ CUtensorMap tm_sfa, const __grid_constant__ CUtensorMap tm_sfb,
                          const __grid_constant__ CUtensorMap tm_out, const Args args) {
@@ -495,7 +547,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     }
     mbar_init(&s.tmem_full[0], 1);
     mbar_init(&s.tmem_full[1], 1);
-    mbar_init(&s.shared_free, 2 * gemm::EPI_WARPS);
+    mbar_init(&s.shared_free, 2 * kEpiWarps);
     mbar_init(&s.drain, 1);
     fence_mbarrier_init();
     prefetch_tensormap(&tm_a);
@@ -565,8 +617,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
       uint32_t phase = 0;
       bool ok = true, any = false;
       for (int tile = pair; ok && tile < num_tiles; tile += npairs, ++local) {
-        // the shared columns of the tile before; its own accumulator's other columns were read
-        // before that tile's epilogue began
+        // the shared columns of the tile before; the other columns of this accumulator were read
+        // before that tile's epilogue began (every warp reports)
         if (local > 0 && !mbar_wait_warp(&s.shared_free, static_cast<uint32_t>(local - 1) & 1u, kStatusTimeoutMma)) break;
         tc_fence_after();
         const int acc = local & 1;
@@ -606,32 +658,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
     const int ew = warp - 2;
+    const int half = ew >> 2;
     const int quarter = warp & 3;
     const int e = threadIdx.x - 64;
     const uint64_t pol_out = policy_evict_first();
     const uint32_t shared_bar = mapa_shared(smem_u32(&s.shared_free), 0);
-    int local = 0, ebuf = 0;
+    int local = 0;
+    bool ok = true;
     for (int tile = pair; tile < num_tiles; tile += npairs, ++local) {
       const int tm = tile / tiles_n;
       const int tn = tile - tm * tiles_n;
       const int acc = local & 1;
       const int row0 = tm * P_BM + rank * 128 + quarter * 32;
+      const int n0 = tn * BN + half * kHalfCols;
+      // the shared columns are the upper half's of accumulator 0 and the lower half's of 1; the other
+      // half (and a warp without rows) only reports that it is done with the tile before
+      const bool shared = row0 < args.M && half != acc;
+      if (!shared && lane == 0) mbar_arrive_cluster(shared_bar);
       stage_params<OUT>(args, tn * BN, e, s.params[acc]);
       const float xs_r = (row0 + lane < args.M && args.xs) ? __ldg(args.xs + row0 + lane) : 1.f;
-      gemm::GatedSlice gs{};
+      GatedSlice gs{};
       if constexpr (OUT == kOutGated) {
-        if (row0 < args.M) gs = gemm::gated_prefetch(args, s.res[ew], s.gate[ew], row0, tn * BN, lane);
+        if (row0 < args.M) gs = gated_prefetch(args, s.epi[ew], s.gate[ew], row0, n0, lane);
       }
-      const bool ok = mbar_wait(&s.tmem_full[acc], static_cast<uint32_t>((local >> 1) & 1), kStatusTimeoutEpilogue);
-      // all four warps staged the parameters; they leave together if any wait ran out
-      if (named_bar_any(1, 128, !ok)) break;
+      // all warps staged the parameters; they leave together if any wait for the tile before ran out
+      if (named_bar_any(1, 32 * kEpiWarps, !ok)) break;
+      ok = mbar_wait_warp(&s.tmem_full[acc], static_cast<uint32_t>((local >> 1) & 1), kStatusTimeoutEpilogue);
       tc_fence_after();
-      if (row0 < args.M) {
-        const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (acc ? 256u - C::kOver : 0u);
-        epilogue_pair<MX, OUT>(args, &tm_out, s, ew, ebuf, gs, t_row, row0, tn * BN, lane, pol_out, xs_r, s.params[acc],
-                               acc == 0, shared_bar);
-      } else if (lane == 0) {
-        mbar_arrive_cluster(shared_bar);
+      if (ok && row0 < args.M) {
+        const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (acc ? 256u - C::kOver : 0u) +
+                               static_cast<uint32_t>(half * kHalfCols);
+        epilogue_pair<MX, OUT>(args, &tm_out, s, ew, half, gs, t_row, row0, n0, lane, pol_out, xs_r, s.params[acc],
+                               shared, shared_bar);
       }
     }
     if constexpr (OUT == kOutGated) cp_async_wait_all();   // a residual copy left by a wait that gave up

@@ -122,7 +122,7 @@ int launch_gemm_fp4_pair(const Fp4Gemm& p, const t8g::gemm4::Args& args, int dev
   const int64_t pairs = std::min<int64_t>(tiles, sms / 2);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs), 1, 1);
-  cfg.blockDim = dim3(NUM_THREADS, 1, 1);
+  cfg.blockDim = dim3(kPairThreads, 1, 1);
   cfg.dynamicSmemBytes = C::kSmemBytes;
   cfg.stream = st;
   cfg.attrs = nullptr;   // the kernel declares its cluster shape (2, 1, 1)

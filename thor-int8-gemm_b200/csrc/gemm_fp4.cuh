@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       int stage = 0, issued = 0;
       uint32_t phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&s.empty[stage], phase ^ 1u, kStatusTimeoutProducer)) break;
+        if (!mbar_wait_sleep(&s.empty[stage], phase ^ 1u, kStatusTimeoutProducer)) break;
         mbar_arrive_expect_tx(&s.full[stage], C::kStageBytes);
         tma_load_2d(s.b[stage], &tm_b, &s.full[stage], kb * BK, tn * TBN, pol_b);
         tma_load_2d(s.sfb[stage], &tm_sfb, &s.full[stage], kb * (C::kSfBytes / 8), tn * TBN / BM, pol_b);
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       // every issued copy must land before the CTA may exit
       for (int i = 0; i < C::kStages && i < issued; ++i) {
         const int n = issued - 1 - i;
-        if (!mbar_wait(&s.full[n % C::kStages], static_cast<uint32_t>((n / C::kStages) & 1), kStatusTimeoutDrain)) break;
+        if (!mbar_wait_sleep(&s.full[n % C::kStages], static_cast<uint32_t>((n / C::kStages) & 1), kStatusTimeoutDrain)) break;
       }
     }
   } else if (warp == 1) {
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     // `done` to the waits' own limits
     mbar_wait_warp(&s.done, 0, kStatusTimeoutDrain);
   } else {
-    have = mbar_wait(&s.done, 0, kStatusTimeoutEpilogue);
+    have = mbar_wait_sleep(&s.done, 0, kStatusTimeoutEpilogue);
     tc_fence_after();
   }
 
@@ -315,6 +315,13 @@ constexpr int kEpiWarps = 8;
 constexpr int kPairThreads = 64 + 32 * kEpiWarps;
 constexpr int kHalfCols = gemm::BN / 2;
 
+// Channel parameters of a tile: weight scales and the bias in the output type.
+template <int OUT>
+struct PairParams {
+  float ws[gemm::BN];
+  uint32_t bias[gemm::BN * OutTraits<OUT>::kBytes / 4];
+};
+
 template <bool MX, int OUT>
 struct PairCfg {
   static constexpr int kTiles = stage_tiles(MX);
@@ -324,7 +331,7 @@ struct PairCfg {
   static constexpr int kSfbBytes = 2 * kTiles * kScaleTile;
   static constexpr int kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;
   static constexpr int kEpiBufs = OUT == kOutGated ? 2 : 1;   // 4 KB pieces per warp (gated: its whole residual slice)
-  static constexpr int kStages = (MX && OUT != kOutGated) ? 5 : 4;
+  static constexpr int kStages = (OUT == kOutGated || (!MX && OUT == kOutF32)) ? 4 : 5;
   static constexpr int kOver = MX ? 32 : 64;             // >= 12 kTiles scale columns
   struct Smem {
     uint8_t a[kStages][kABytes];
@@ -333,7 +340,7 @@ struct PairCfg {
     uint8_t gate[kEpiWarps][OUT == kOutGated ? 2 * kHalfCols : 16];
     alignas(128) uint8_t sfa[kStages][kSfaBytes];
     alignas(128) uint8_t sfb[kStages][kSfbBytes];
-    gemm::TileParams params[2];
+    PairParams<OUT> params[2];
     uint64_t full[kStages];
     uint64_t empty[kStages];
     uint64_t tmem_full[2];
@@ -346,19 +353,17 @@ struct PairCfg {
   static_assert(12 * kTiles <= kOver, "the scales fit the columns between the accumulators");
 };
 
-// ws (1 without weight scales) and bias of the tile's columns; 2-byte outputs take the bias as packed
-// pairs of the output type.
+// ws (1 without weight scales) and bias (0 without one) of the tile's columns.
 template <int OUT>
-__device__ __forceinline__ void stage_params(const Args& args, int n_tile0, int e, gemm::TileParams& tp) {
+__device__ __forceinline__ void stage_params(const Args& args, int n_tile0, int e, PairParams<OUT>& tp) {
   static_assert(gemm::BN == 32 * kEpiWarps, "one column per epilogue thread");
   const int n = n_tile0 + e;
   const bool in = n < args.N;
   tp.ws[e] = args.ws == nullptr ? 1.f : in ? __ldg(args.ws + (args.ws_stride ? n : 0)) : 0.f;
-  if constexpr (OUT == kOutF32) {
-    tp.bias[e] = (in && args.bias) ? static_cast<const float*>(args.bias)[n] : 0.f;
-  } else {
-    reinterpret_cast<uint16_t*>(tp.bias2)[e] = (in && args.bias) ? static_cast<const uint16_t*>(args.bias)[n] : 0;
-  }
+  if constexpr (OUT == kOutF32)
+    tp.bias[e] = (in && args.bias) ? static_cast<const uint32_t*>(args.bias)[n] : 0u;
+  else
+    reinterpret_cast<uint16_t*>(tp.bias)[e] = (in && args.bias) ? static_cast<const uint16_t*>(args.bias)[n] : 0;
 }
 
 // Gated form: the residual rows of a warp's 32 x 128 slice are copied into its staging pieces (the
@@ -412,7 +417,7 @@ template <bool MX, int OUT>
 __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMap* tm_out,
                                               typename PairCfg<MX, OUT>::Smem& s, int ew, int half,
                                               const GatedSlice& gs, uint32_t t_row, int row0, int n0, int lane,
-                                              uint64_t pol_out, float xs_r, const gemm::TileParams& tp, bool shared,
+                                              uint64_t pol_out, float xs_r, const PairParams<OUT>& tp, bool shared,
                                               uint32_t shared_bar) {
   constexpr int kCols = OUT == kOutF32 ? 32 : 64;
   constexpr int kChunks = kHalfCols / kCols;
@@ -442,14 +447,14 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
     if (shared && i == kFirst - 1) {   // the next tile's MMAs wait for this
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(shared_bar);
+      if (lane == 0) mbar_arrive_cluster_relaxed(shared_bar);
     }
     if (i + 1 < kChunks) load(i + 1);
     if (c * kCols >= cols) continue;
     const float4* wq = reinterpret_cast<const float4*>(tp.ws + half * kHalfCols + c * kCols);
     uint8_t* buf = s.epi[ew][OUT == kOutGated ? c : 0];
     if constexpr (OUT == kOutGated) {
-      const uint4* bq2 = reinterpret_cast<const uint4*>(tp.bias2 + (half * kHalfCols + c * kCols) / 2);
+      const uint4* bq2 = reinterpret_cast<const uint4*>(tp.bias + (half * kHalfCols + c * kCols) / 2);
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         const float4 w0 = wq[2 * q], w1 = wq[2 * q + 1];
@@ -477,25 +482,26 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
         *cell = make_uint4(o[0], o[1], o[2], o[3]);
       }
     } else {
-      const float4* bq = reinterpret_cast<const float4*>(tp.bias + half * kHalfCols + c * kCols);
-      const uint4* bq2 = reinterpret_cast<const uint4*>(tp.bias2 + (half * kHalfCols + c * kCols) / 2);
+      // eight 16-byte pieces of the row: four fp32 or eight two-byte outputs each
+      const uint4* bq = reinterpret_cast<const uint4*>(tp.bias + (half * kHalfCols + c * kCols) * OutTraits<OUT>::kBytes / 4);
       uint4 o[8];
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         if constexpr (OUT == kOutF32) {
-          const float4 w4 = wq[q], b4 = bq[q];
+          const float4 w4 = wq[q];
+          const uint4 b4 = bq[q];
           float2 f0 = mul2_rn(mul2_rn(make_float2(v[4 * q], v[4 * q + 1]), xs2), make_float2(w4.x, w4.y));
           float2 f1 = mul2_rn(mul2_rn(make_float2(v[4 * q + 2], v[4 * q + 3]), xs2), make_float2(w4.z, w4.w));
           if (has_bias) {
-            f0 = make_float2(__fadd_rn(f0.x, b4.x), __fadd_rn(f0.y, b4.y));
-            f1 = make_float2(__fadd_rn(f1.x, b4.z), __fadd_rn(f1.y, b4.w));
+            f0 = make_float2(__fadd_rn(f0.x, __uint_as_float(b4.x)), __fadd_rn(f0.y, __uint_as_float(b4.y)));
+            f1 = make_float2(__fadd_rn(f1.x, __uint_as_float(b4.z)), __fadd_rn(f1.y, __uint_as_float(b4.w)));
           }
           o[q] = make_uint4(__float_as_uint(f0.x), __float_as_uint(f0.y), __float_as_uint(f1.x), __float_as_uint(f1.y));
         } else {
           const float4 w0 = wq[2 * q], w1 = wq[2 * q + 1];
           const float2 wp[4] = {make_float2(w0.x, w0.y), make_float2(w0.z, w0.w), make_float2(w1.x, w1.y),
                                 make_float2(w1.z, w1.w)};
-          const uint4 b4 = has_bias ? bq2[q] : make_uint4(0, 0, 0, 0);
+          const uint4 b4 = has_bias ? bq[q] : make_uint4(0, 0, 0, 0);
           const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w};
           uint32_t h[4];
 #pragma unroll
@@ -578,7 +584,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const int tm = tile / tiles_n;
         const int tn = tile - tm * tiles_n;
         for (int kb = 0; kb < args.kstages; ++kb) {
-          if (!mbar_wait(&s.empty[stage], phase ^ 1u, kStatusTimeoutProducer)) {
+          if (!mbar_wait_sleep(&s.empty[stage], phase ^ 1u, kStatusTimeoutProducer)) {
             ok = false;
             break;
           }
@@ -599,7 +605,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       if (rank == 0) {
         for (int i = 0; i < C::kStages && i < issued; ++i) {
           const int n = issued - 1 - i;
-          if (!mbar_wait(&s.full[n % C::kStages], static_cast<uint32_t>((n / C::kStages) & 1), kStatusTimeoutDrain)) break;
+          if (!mbar_wait_sleep(&s.full[n % C::kStages], static_cast<uint32_t>((n / C::kStages) & 1), kStatusTimeoutDrain)) break;
         }
       }
     }
@@ -674,7 +680,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       // the shared columns are the upper half's of accumulator 0 and the lower half's of 1; the other
       // half (and a warp without rows) only reports that it is done with the tile before
       const bool shared = row0 < args.M && half != acc;
-      if (!shared && lane == 0) mbar_arrive_cluster(shared_bar);
+      if (!shared && lane == 0) mbar_arrive_cluster_relaxed(shared_bar);
       stage_params<OUT>(args, tn * BN, e, s.params[acc]);
       const float xs_r = (row0 + lane < args.M && args.xs) ? __ldg(args.xs + row0 + lane) : 1.f;
       GatedSlice gs{};

@@ -474,9 +474,45 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
-// mbar_wait by a whole warp that stays together: false in every lane if any lane's wait ran out.
+// mbar_wait that sleeps in the barrier for up to 20 us a try instead of the default limit, so that
+// many waiting warps neither poll shared memory (whose cycles the tensor cores' operands need) nor
+// sit in a read of %globaltimer when the phase completes.
+__device__ __forceinline__ bool mbar_wait_sleep(uint64_t* bar, uint32_t parity, int code) {
+  const uint32_t a = smem_u32(bar);
+  if (mbar_try_wait(a, parity)) return true;
+  uint64_t t0 = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        "  .reg .pred p;\n"
+        "  mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        "  selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(a), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+    const uint64_t t = globaltimer_ns();
+    if (t0 == 0) {
+      t0 = t;
+    } else if (t - t0 > kWaitLimitNs) {
+      record_status(code);
+      return false;
+    }
+  }
+}
+
+// The same by a whole warp that stays together: false in every lane if any lane's wait ran out.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int code) {
-  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, code));
+  return __all_sync(0xFFFFFFFFu, mbar_wait_sleep(bar, parity, code));
+}
+
+// Arrive anywhere in the cluster without ordering this thread's memory accesses: enough to hand TMEM
+// columns over (their loads are complete and a tcgen05 fence precedes it), and it does not wait
+// for the thread's outstanding stores as a cluster-scope release does.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 }  // namespace t8g

@@ -613,8 +613,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     // ------------------------------------------------------------ MMA issuer (leader only)
     if (rank == 0) {
       constexpr uint32_t idesc = make_idesc_fp4(MX, P_BM, BN);
-      const uint32_t empty0[2] = {mapa_shared(smem_u32(&s.empty[0]), 0), mapa_shared(smem_u32(&s.empty[0]), 1)};
-      const uint32_t tfull0[2] = {mapa_shared(smem_u32(&s.tmem_full[0]), 0), mapa_shared(smem_u32(&s.tmem_full[0]), 1)};
       const uint32_t sa_t = tmem_base + 512u - C::kOver;
       const uint32_t sb_t = sa_t + 4u * C::kTiles;
       const StageDescs d0 = {smem_desc_k_sw128(smem_u32(s.a[0])), smem_desc_k_sw128(smem_u32(s.b[0])),
@@ -640,12 +638,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                                   d0.sfa + stage * (C::kSfaBytes / 16), d0.sfb + stage * (C::kSfbBytes / 16)};
             stage_mmas<MX, true, 2>(d_tmem, d, sa_t, sb_t, 0u, idesc,
                                     kb == args.kstages - 1 ? args.last_steps : kStageK / kMmaK, kb != 0);
-            tc_commit_pair(empty0[0] + 8u * static_cast<uint32_t>(stage));
-            tc_commit_pair(empty0[1] + 8u * static_cast<uint32_t>(stage));
-            if (kb == args.kstages - 1) {
-              tc_commit_pair(tfull0[0] + 8u * static_cast<uint32_t>(acc));
-              tc_commit_pair(tfull0[1] + 8u * static_cast<uint32_t>(acc));
-            }
+            tc_commit_both(smem_u32(&s.empty[stage]));
+            if (kb == args.kstages - 1) tc_commit_both(smem_u32(&s.tmem_full[acc]));
           }
           __syncwarp();
           any = true;

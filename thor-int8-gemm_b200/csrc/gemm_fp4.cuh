@@ -88,67 +88,95 @@ __device__ __forceinline__ void stage_mmas(uint32_t d_tmem, const StageDescs& d,
     stage_mmas_n<MX, PAIR, B_GROUPS, 1>(d_tmem, d, sa_t, sb_t, sb_off, idesc, accumulate);
 }
 
-// ---------------------------------------------------------------- epilogue arithmetic
-// One output element from its accumulator, in the 8-bit GEMMs' operation order.
+// ---------------------------------------------------------------- 1-SM kernel
+// For outputs of few tiles: one 128 x TBN tile per cluster of S CTAs (1..8) that split K.  Each CTA
+// leaves its partial tile in its shared memory; the tile's pieces of eight columns are dealt over
+// the threads of all S CTAs, and a thread sums its pieces over the partial tiles in rank
+// order (a fixed order, so results repeat) through distributed shared memory.
+// A tile has `arows` rows of A to load (the rows of M, a multiple of 8): a box that reaches past M
+// by most of its rows loads several times slower, and its slot would hold nothing.  The MMA
+// still reads 128 rows, whatever the ring holds there: those rows' sums are not stored.
+// About 104 KB a CTA, so that two share an SM and one's start and end overlap the other's stream.
+constexpr int kSmallMaxStages = 16;
+constexpr uint32_t kSmallSmem = 104 * 1024;
+
+template <bool MX, int TBN>
+struct SmallCfg {
+  static constexpr uint32_t kTiles = stage_tiles(MX);
+  static constexpr uint32_t kBBytes = TBN * BK;
+  static constexpr uint32_t kSfBytes = kTiles * kScaleTile;   // per operand (one 128-row group)
+  static constexpr uint32_t kSfCols = 2u * 4u * kTiles;       // A's and B's scale columns of a stage
+  static constexpr uint32_t kTmemCols = TBN + 2 * kSfCols <= 128 ? 128 : 256;   // scales double-buffered
+  static constexpr uint32_t kPitch = TBN + 4;                 // floats per row of a partial tile
+  __host__ __device__ static constexpr uint32_t stage_bytes(uint32_t arows) { return arows * BK + kBBytes + 2 * kSfBytes; }
+  __host__ __device__ static constexpr uint32_t partial_bytes(uint32_t rows) { return rows * kPitch * 4; }
+};
+
+// Eight output columns [n, n + 8) of row m from their sums (fewer at the right edge).
 template <int OUT>
-__device__ __forceinline__ void store_one(const Args& a, int m, int n, float acc, float xs_r, int64_t grow) {
-  float f = __fmul_rn(acc, xs_r);
-  f = __fmul_rn(f, a.ws ? __ldg(a.ws + (a.ws_stride ? n : 0)) : 1.f);
-  if (a.bias != nullptr) f = __fadd_rn(f, OutTraits<OUT>::to_f32(a.bias, n));
+__device__ __forceinline__ void store_eight(const Args& a, int m, int n, float (&f)[8]) {
+  const float xs = a.xs ? __ldg(a.xs + m) : 1.f;
+  const int left = a.N - n;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int c = min(n + j, a.N - 1);
+    f[j] = __fmul_rn(__fmul_rn(f[j], xs), a.ws ? __ldg(a.ws + (a.ws_stride ? c : 0)) : 1.f);
+    if (a.bias != nullptr) f[j] = __fadd_rn(f[j], OutTraits<OUT>::to_f32(a.bias, c));
+  }
   const int64_t at = static_cast<int64_t>(m) * a.ld_out + n;
   if constexpr (OUT == kOutF32) {
-    static_cast<float*>(a.out)[at] = f;
-  } else if constexpr (OUT == kOutF16) {
-    static_cast<__half*>(a.out)[at] = __float2half_rn(f);
-  } else if constexpr (OUT == kOutBF16) {
-    static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(f);
+    float* o = static_cast<float*>(a.out) + at;
+    if (left >= 8) {
+      reinterpret_cast<float4*>(o)[0] = make_float4(f[0], f[1], f[2], f[3]);
+      reinterpret_cast<float4*>(o)[1] = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < left) o[j] = f[j];
+    }
   } else {
-    const float g = __bfloat162float(static_cast<const __nv_bfloat16*>(a.gate)[grow * a.ld_gate + n]);
-    const float r = __bfloat162float(static_cast<const __nv_bfloat16*>(a.res)[static_cast<int64_t>(m) * a.ld_res + n]);
-    static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(__fmaf_rn(g, f, r));
+    if constexpr (OUT == kOutGated) {   // N is a multiple of 8
+      const int64_t grow = a.gate_index ? static_cast<int64_t>(__ldg(a.gate_index + m)) : m / a.rows_per_gate;
+      const uint4 g4 = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.gate) + grow * a.ld_gate + n));
+      // res may be out itself: an ordinary load
+      const uint4 r4 = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.res) + static_cast<int64_t>(m) * a.ld_res + n);
+      const uint32_t gw[4] = {g4.x, g4.y, g4.z, g4.w}, rw[4] = {r4.x, r4.y, r4.z, r4.w};
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const float2 o = fma2_rn(bf2_to_f2(gw[p]), make_float2(f[2 * p], f[2 * p + 1]), bf2_to_f2(rw[p]));
+        f[2 * p] = o.x;
+        f[2 * p + 1] = o.y;
+      }
+    }
+    uint32_t h[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) h[p] = OutTraits<OUT>::pack2(f[2 * p], f[2 * p + 1]);
+    uint16_t* o = static_cast<uint16_t*>(a.out) + at;
+    if (left >= 8) {
+      *reinterpret_cast<uint4*>(o) = make_uint4(h[0], h[1], h[2], h[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < left) o[j] = static_cast<uint16_t>(h[j / 2] >> (16 * (j & 1)));
+    }
   }
 }
 
-// ---------------------------------------------------------------- 1-SM kernel
-// One 128 x TBN output tile per cluster of gridDim-given size S (1..8): the S CTAs split K, each
-// leaves its partial tile in its own shared memory, and CTA r sums columns [r, r + 1) * TBN / S of
-// all partials in rank order (a fixed order, so results repeat) and stores them.
-template <bool MX, int TBN>
-struct Cfg {
-  static constexpr int kTiles = stage_tiles(MX);
-  static constexpr int kABytes = BM * BK;
-  static constexpr int kBBytes = TBN * BK;
-  static constexpr int kSfBytes = kTiles * kScaleTile;   // per operand (one 128-row group)
-  static constexpr int kStageBytes = kABytes + kBBytes + 2 * kSfBytes;
-  static constexpr int kStages = (200 * 1024) / kStageBytes;
-  static constexpr uint32_t kSfCols = 2u * 4u * kTiles;  // A's and B's scale columns of a stage
-  static constexpr uint32_t kTmemCols = TBN + 2 * kSfCols <= 128 ? 128 : 256;   // scales double-buffered
-  static constexpr int kPitch = TBN + 1;                 // floats per row of a partial tile
-  struct Smem {
-    uint8_t a[kStages][kABytes];
-    uint8_t b[kStages][kBBytes];
-    alignas(1024) uint8_t sfa[kStages][kSfBytes];
-    uint8_t sfb[kStages][kSfBytes];
-    uint64_t full[kStages];
-    uint64_t empty[kStages];
-    uint64_t done;
-    uint64_t drain;
-    uint32_t tmem_base;
-  };
-  static constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
-  static_assert(kSmemBytes <= 227 * 1024, "shared memory");
-  static_assert(static_cast<int>(sizeof(float)) * BM * kPitch <= kStages * kABytes, "partial tile fits the A ring");
-};
-
 template <bool MX, int OUT, int TBN>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+__global__ void __launch_bounds__(NUM_THREADS, 2)
     gemm_fp4_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                     const __grid_constant__ CUtensorMap tm_sfa, const __grid_constant__ CUtensorMap tm_sfb,
-                    const Args args, const int S) {
+                    const Args args, const int S, const uint32_t arows, const int stages) {
   extern __shared__ uint8_t smem_raw[];
-  using C = Cfg<MX, TBN>;
-  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
-  typename C::Smem& s = *reinterpret_cast<typename C::Smem*>(smem_raw + pad);
+  __shared__ uint64_t full[kSmallMaxStages], empty[kSmallMaxStages], done;
+  __shared__ uint32_t tmem_slot;
+  using C = SmallCfg<MX, TBN>;
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  // rings: A, B, A's scales, B's scales (every slot a multiple of 1024 bytes)
+  const uint32_t a_bytes = arows * BK;
+  uint8_t* ring_b = smem + stages * a_bytes;
+  uint8_t* ring_sfa = ring_b + stages * C::kBBytes;
+  uint8_t* ring_sfb = ring_sfa + stages * C::kSfBytes;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int rank = static_cast<int>(blockIdx.x) % S;
@@ -160,21 +188,25 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   const int kb1 = static_cast<int>(static_cast<int64_t>(args.kstages) * (rank + 1) / S);
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], 1);
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
     }
-    mbar_init(&s.done, 1);
+    mbar_init(&done, 1);
     fence_mbarrier_init();
+    prefetch_tensormap(&tm_a);
+    prefetch_tensormap(&tm_b);
+    prefetch_tensormap(&tm_sfa);
+    prefetch_tensormap(&tm_sfb);
   }
   if (warp == 1) {
-    tmem_alloc(&s.tmem_base, C::kTmemCols);
+    tmem_alloc(&tmem_slot, C::kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = s.tmem_base;
+  const uint32_t tmem_base = tmem_slot;
 
   bool have = false;   // epilogue warps: the accumulator is complete
   if (warp == 0) {
@@ -184,110 +216,114 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       int stage = 0, issued = 0;
       uint32_t phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait_sleep(&s.empty[stage], phase ^ 1u, kStatusTimeoutProducer)) break;
-        mbar_arrive_expect_tx(&s.full[stage], C::kStageBytes);
-        tma_load_2d(s.b[stage], &tm_b, &s.full[stage], kb * BK, tn * TBN, pol_b);
-        tma_load_2d(s.sfb[stage], &tm_sfb, &s.full[stage], kb * (C::kSfBytes / 8), tn * TBN / BM, pol_b);
-        tma_load_2d(s.a[stage], &tm_a, &s.full[stage], kb * BK, tm * BM, pol_a);
-        tma_load_2d(s.sfa[stage], &tm_sfa, &s.full[stage], kb * (C::kSfBytes / 8), tm, pol_a);
+        if (!mbar_wait_sleep(&empty[stage], phase ^ 1u, kStatusTimeoutProducer)) break;
+        mbar_arrive_expect_tx(&full[stage], C::stage_bytes(arows));
+        tma_load_2d(ring_b + stage * C::kBBytes, &tm_b, &full[stage], kb * BK, tn * TBN, pol_b);
+        tma_load_2d(ring_sfb + stage * C::kSfBytes, &tm_sfb, &full[stage], kb * (static_cast<int>(C::kSfBytes) / 8),
+                    tn * TBN / BM, pol_b);
+        tma_load_2d(smem + stage * a_bytes, &tm_a, &full[stage], kb * BK, tm * BM, pol_a);
+        tma_load_2d(ring_sfa + stage * C::kSfBytes, &tm_sfa, &full[stage], kb * (static_cast<int>(C::kSfBytes) / 8), tm,
+                    pol_a);
         ++issued;
-        if (++stage == C::kStages) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
       }
       // every issued copy must land before the CTA may exit
-      for (int i = 0; i < C::kStages && i < issued; ++i) {
+      for (int i = 0; i < stages && i < issued; ++i) {
         const int n = issued - 1 - i;
-        if (!mbar_wait_sleep(&s.full[n % C::kStages], static_cast<uint32_t>((n / C::kStages) & 1), kStatusTimeoutDrain)) break;
+        if (!mbar_wait_sleep(&full[n % stages], static_cast<uint32_t>((n / stages) & 1), kStatusTimeoutDrain)) break;
       }
     }
   } else if (warp == 1) {
     constexpr uint32_t idesc = make_idesc_fp4(MX, BM, TBN);
     const uint32_t sb_off = static_cast<uint32_t>(tn * TBN % BM / 32);
-    const StageDescs d0 = {smem_desc_k_sw128(smem_u32(s.a[0])), smem_desc_k_sw128(smem_u32(s.b[0])),
-                           smem_desc_scales(smem_u32(s.sfa[0])), smem_desc_scales(smem_u32(s.sfb[0]))};
+    const StageDescs d0 = {smem_desc_k_sw128(smem_u32(smem)), smem_desc_k_sw128(smem_u32(ring_b)),
+                           smem_desc_scales(smem_u32(ring_sfa)), smem_desc_scales(smem_u32(ring_sfb))};
     int stage = 0;
     uint32_t phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
-      if (!mbar_wait_warp(&s.full[stage], phase, kStatusTimeoutMma)) break;
+      if (!mbar_wait_warp(&full[stage], phase, kStatusTimeoutMma)) break;
       tc_fence_after();
       if (elect_one()) {
         const uint32_t sa_t = tmem_base + TBN + static_cast<uint32_t>(kb & 1) * C::kSfCols;
-        const StageDescs d = {d0.a + stage * (C::kABytes / 16), d0.b + stage * (C::kBBytes / 16),
-                              d0.sfa + stage * (C::kSfBytes / 16), d0.sfb + stage * (C::kSfBytes / 16)};
+        const uint32_t i = static_cast<uint32_t>(stage);
+        const StageDescs d = {d0.a + i * (a_bytes / 16), d0.b + i * (C::kBBytes / 16), d0.sfa + i * (C::kSfBytes / 16),
+                              d0.sfb + i * (C::kSfBytes / 16)};
         stage_mmas<MX, false, 1>(tmem_base, d, sa_t, sa_t + 4u * C::kTiles, sb_off, idesc,
                                  kb == args.kstages - 1 ? args.last_steps : kStageK / kMmaK, kb != kb0);
-        tc_commit(&s.empty[stage]);
-        if (kb == kb1 - 1) tc_commit(&s.done);
+        tc_commit(&empty[stage]);
+        if (kb == kb1 - 1) tc_commit(&done);
       }
       __syncwarp();
-      if (++stage == C::kStages) {
+      if (++stage == stages) {
         stage = 0;
         phase ^= 1u;
       }
     }
     // every MMA (and its shared-memory reads) completes before teardown; a wait that gave up leaves
     // `done` to the waits' own limits
-    mbar_wait_warp(&s.done, 0, kStatusTimeoutDrain);
+    mbar_wait_warp(&done, 0, kStatusTimeoutDrain);
   } else {
-    have = mbar_wait_sleep(&s.done, 0, kStatusTimeoutEpilogue);
+    have = mbar_wait_warp(&done, 0, kStatusTimeoutEpilogue);
     tc_fence_after();
   }
 
+  // The rings' slots are all consumed once `done` completed: the partial tile goes there.
+  float* part = reinterpret_cast<float*>(smem);
+  const int rows = min(BM, args.M - tm * BM);
   const int quarter = warp & 3;
-  const int row = quarter * 32 + lane;
-  const int m = tm * BM + row;
-  const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-  if (S == 1) {
-    if (warp >= 2 && have) {
-      const float xs_r = (m < args.M && args.xs) ? __ldg(args.xs + m) : 1.f;
-      const int64_t grow = (OUT == kOutGated && m < args.M) ? (args.gate_index ? args.gate_index[m] : m / args.rows_per_gate) : 0;
-      for (int c = 0; c < TBN; c += EPI_COLS) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(t_row + static_cast<uint32_t>(c), r);
-        tmem_ld_wait_regs(r);
-        if (m < args.M) {
+  if (warp >= 2 && quarter * 32 < rows) {
+    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    float* prow = part + static_cast<uint32_t>(quarter * 32 + lane) * C::kPitch;
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (tn * TBN + c + j < args.N) store_one<OUT>(args, m, tn * TBN + c + j, __uint_as_float(r[j]), xs_r, grow);
+    for (int c = 0; c < TBN; c += 32) {
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(t_row + static_cast<uint32_t>(c), r);
+      tmem_ld_wait_regs(r);
+      if (quarter * 32 + lane < rows) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+          *reinterpret_cast<uint4*>(prow + c + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+      }
+    }
+  }
+  __syncwarp();
+  if (S > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  if (warp >= 2 && have) {
+    constexpr int kPieces = TBN / 8;
+    for (int u = rank * 128 + static_cast<int>(threadIdx.x) - 64; u < rows * kPieces; u += S * 128) {
+      const int rr = u / kPieces;
+      const int cc = (u - rr * kPieces) * 8;
+      const int n = tn * TBN + cc;
+      if (n >= args.N) continue;
+      const float* at = part + static_cast<uint32_t>(rr) * C::kPitch + cc;
+      float f[8];
+      if (S == 1) {
+        const float4 lo = reinterpret_cast<const float4*>(at)[0], hi = reinterpret_cast<const float4*>(at)[1];
+        f[0] = lo.x, f[1] = lo.y, f[2] = lo.z, f[3] = lo.w, f[4] = hi.x, f[5] = hi.y, f[6] = hi.z, f[7] = hi.w;
+      } else {
+        const uint32_t addr = smem_u32(at);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = 0.f;
+#pragma unroll 4
+        for (int q = 0; q < S; ++q) {
+          const uint32_t p = mapa_shared(addr, static_cast<uint32_t>(q));
+          const float4 lo = ld_cluster_f32x4(p), hi = ld_cluster_f32x4(p + 16);
+          f[0] = __fadd_rn(f[0], lo.x), f[1] = __fadd_rn(f[1], lo.y), f[2] = __fadd_rn(f[2], lo.z);
+          f[3] = __fadd_rn(f[3], lo.w), f[4] = __fadd_rn(f[4], hi.x), f[5] = __fadd_rn(f[5], hi.y);
+          f[6] = __fadd_rn(f[6], hi.z), f[7] = __fadd_rn(f[7], hi.w);
         }
       }
+      store_eight<OUT>(args, tm * BM + rr, n, f);
     }
-  } else {
-    // the A ring's stages are all consumed once `done` completed: the partial tile goes there
-    float* part = reinterpret_cast<float*>(s.a);
-    if (warp >= 2) {
-      for (int c = 0; c < TBN; c += EPI_COLS) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(t_row + static_cast<uint32_t>(c), r);
-        tmem_ld_wait_regs(r);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) part[row * C::kPitch + c + j] = __uint_as_float(r[j]);
-      }
-    }
-    __syncwarp();
-    cluster_sync();
-    if (warp >= 2 && have) {
-      const int e = threadIdx.x - 64;
-      const int cols = TBN / S;
-      const int rows = min(BM, args.M - tm * BM);
-      for (int i = e; i < rows * cols; i += 128) {
-        const int rr = i / cols;
-        const int cc = rank * cols + (i - rr * cols);
-        const int n = tn * TBN + cc;
-        if (n >= args.N) continue;
-        const uint32_t at = smem_u32(part + rr * C::kPitch + cc);
-        float acc = 0.f;
-        for (int q = 0; q < S; ++q) acc = __fadd_rn(acc, ld_cluster_f32(mapa_shared(at, static_cast<uint32_t>(q))));
-        const int mm = tm * BM + rr;
-        const int64_t grow = OUT == kOutGated ? (args.gate_index ? args.gate_index[mm] : mm / args.rows_per_gate) : 0;
-        store_one<OUT>(args, mm, n, acc, args.xs ? __ldg(args.xs + mm) : 1.f, grow);
-      }
-    }
-    __syncwarp();
-    cluster_sync();   // no CTA leaves while another reads its partial tile
   }
+  __syncwarp();
+  if (S > 1) cluster_sync();   // no CTA leaves while another reads its partial tile
 
   tc_fence_before();
   __syncthreads();
@@ -296,7 +332,6 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     tmem_dealloc(tmem_base, C::kTmemCols);
   }
 }
-
 
 // ---------------------------------------------------------------- 2-SM kernel
 // The 8-bit pair kernel's scheme (gemm.cuh): a cluster of two CTAs computes 256 x 256 tiles with

@@ -452,10 +452,13 @@ __device__ __forceinline__ uint64_t smem_desc_scales(uint32_t smem_addr) {
   return d;
 }
 
-// A float at `addr`, an address of the cluster's shared memory (mapa_shared).
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+// Four floats at `addr`, an address of the cluster's shared memory (mapa_shared).
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 

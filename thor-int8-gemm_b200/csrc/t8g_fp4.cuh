@@ -53,15 +53,16 @@ struct Fp4Gemm {
 template <bool MX, int OUT, int TBN>
 int launch_gemm_fp4_small(const Fp4Gemm& p, const t8g::gemm4::Args& args, int split, int dev, cudaStream_t st) {
   using namespace t8g::gemm4;
-  using C = Cfg<MX, TBN>;
+  using C = SmallCfg<MX, TBN>;
   static std::atomic<bool> attr_done[kMaxDevices] = {};
   auto kern = gemm_fp4_kernel<MX, OUT, TBN>;
-  int rc = ensure_smem_attr(kern, dev, C::kSmemBytes, attr_done);
+  int rc = ensure_smem_attr(kern, dev, kSmallSmem, attr_done);
   if (rc) return rc;
   const int64_t words = fp4_words(p.K, p.kind);
   const uint32_t sf_box = C::kSfBytes / 8;   // a stage's scale tiles of a row group, as 8-byte elements
+  const uint32_t arows = static_cast<uint32_t>(std::min<int64_t>((p.M + 7) / 8 * 8, BM));
   CUtensorMap ta, tb, tsa, tsb;
-  if ((rc = encode_2d(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.x, p.K / 2, p.M, p.ld_x, BK, BM, CU_TENSOR_MAP_SWIZZLE_128B)))
+  if ((rc = encode_2d(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.x, p.K / 2, p.M, p.ld_x, BK, arows, CU_TENSOR_MAP_SWIZZLE_128B)))
     return rc;
   if ((rc = encode_2d(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.w, p.K / 2, p.N, p.ld_w, BK, TBN, CU_TENSOR_MAP_SWIZZLE_128B)))
     return rc;
@@ -73,10 +74,15 @@ int launch_gemm_fp4_small(const Fp4Gemm& p, const t8g::gemm4::Args& args, int sp
     return rc;
   const int64_t tiles = ((p.M + BM - 1) / BM) * ((p.N + TBN - 1) / TBN);
   if (tiles * split >= (int64_t(1) << 31)) return fail(T8G_ERR_UNSUPPORTED, "gemm_fp4: too many tiles");
+  // as many stages as fit, at least two (the MMA reads 16 KB from the start of any A slot: the B ring
+  // behind the A ring holds that much)
+  const int stages = static_cast<int>(std::min<uint32_t>((kSmallSmem - 1024) / C::stage_bytes(arows), kSmallMaxStages));
+  static_assert(2 * C::stage_bytes(BM) + 1024 <= kSmallSmem && 2 * C::kBBytes >= 128 * BK, "two stages fit");
+  static_assert(C::partial_bytes(BM) + 1024 <= kSmallSmem, "a partial tile fits");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles * split), 1, 1);
   cfg.blockDim = dim3(NUM_THREADS, 1, 1);
-  cfg.dynamicSmemBytes = C::kSmemBytes;
+  cfg.dynamicSmemBytes = kSmallSmem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -85,7 +91,7 @@ int launch_gemm_fp4_small(const Fp4Gemm& p, const t8g::gemm4::Args& args, int sp
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  T8G_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, ta, tb, tsa, tsb, args, split), "gemm_fp4 launch");
+  T8G_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, ta, tb, tsa, tsb, args, split, arows, stages), "gemm_fp4 launch");
   return T8G_OK;
 }
 
@@ -138,7 +144,7 @@ int launch_gemm_fp4(const Fp4Gemm& p, const t8g::gemm4::Args& args, int dev, int
   const bool narrow = tm * ((p.N + 127) / 128) < sms;
   const int64_t tiles = tm * ((p.N + (narrow ? 63 : 127)) / (narrow ? 64 : 128));
   int split = 1;
-  while (split < 8 && tiles * split * 2 <= sms && args.kstages >= 4 * split) split *= 2;
+  while (split < 8 && tiles * split * 2 <= 2 * sms && args.kstages >= 6 * split) split *= 2;
   return narrow ? launch_gemm_fp4_small<MX, OUT, 64>(p, args, split, dev, st)
                 : launch_gemm_fp4_small<MX, OUT, 128>(p, args, split, dev, st);
 }

@@ -137,16 +137,34 @@ int launch_gemm_fp4_pair(const Fp4Gemm& p, const t8g::gemm4::Args& args, int dev
   return T8G_OK;
 }
 
+// Which kernel, tile width and split (device times of one call, nvfp4, on a B200 with 148 SMs):
+//   the pair kernel has a floor of 7 to 10 us and then the full rate; it runs above 64 rows when its
+//   256 x 256 tiles occupy more than a quarter of the SMs (128 x 9216 x 3072: 10.2 us, 11.9 with the small
+//   kernel), and above 128 rows also when K is too short to be worth splitting (at most 8 stages:
+//   256 x 1024 x 1024 7.5 us against 8.3, but 256 x 3072 x 12288 20.5 against 18.3);
+//   the small kernel takes the tile width and the power-of-two split that bring the CTAs nearest to
+//   one an SM (1 x 9216 x 3072: 72 tiles x 2 7.3 us, x 1 8.5, x 4 10.5; 1 x 3072 x 3072: 24 x 4 5.8,
+//   x 8 6.6), 128 columns where both widths come equally near (1 x 9216 x 3072: 144 x 1 of 64 columns
+//   9.5), 64 above 64 rows, where the partial tiles' sums weigh more (128 x 3072 x 3072: 9.6, 10.0).
+struct SmallPlan {
+  int64_t ctas;
+  int split;
+};
+SmallPlan small_plan(int64_t M, int64_t N, int tbn, int kstages, int sms) {
+  const int64_t tiles = (M + 127) / 128 * ((N + tbn - 1) / tbn);
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= sms && split * 2 <= kstages) split *= 2;
+  return {std::min<int64_t>(tiles * split, sms), split};
+}
+
 template <bool MX, int OUT>
 int launch_gemm_fp4(const Fp4Gemm& p, const t8g::gemm4::Args& args, int dev, int sms, cudaStream_t st) {
-  if (((p.M + 255) / 256) * ((p.N + 255) / 256) * 4 >= sms) return launch_gemm_fp4_pair<MX, OUT>(p, args, dev, sms, st);
-  const int64_t tm = (p.M + 127) / 128;
-  const bool narrow = tm * ((p.N + 127) / 128) < sms;
-  const int64_t tiles = tm * ((p.N + (narrow ? 63 : 127)) / (narrow ? 64 : 128));
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= 2 * sms && args.kstages >= 6 * split) split *= 2;
-  return narrow ? launch_gemm_fp4_small<MX, OUT, 64>(p, args, split, dev, st)
-                : launch_gemm_fp4_small<MX, OUT, 128>(p, args, split, dev, st);
+  const bool many = (p.M + 255) / 256 * ((p.N + 255) / 256) * 8 > sms;
+  if ((p.M > 64 && many) || (p.M > 128 && args.kstages <= 8)) return launch_gemm_fp4_pair<MX, OUT>(p, args, dev, sms, st);
+  const SmallPlan w = small_plan(p.M, p.N, 128, args.kstages, sms), n = small_plan(p.M, p.N, 64, args.kstages, sms);
+  if (n.ctas > w.ctas || (n.ctas == w.ctas && p.M > 64))
+    return launch_gemm_fp4_small<MX, OUT, 64>(p, args, n.split, dev, st);
+  return launch_gemm_fp4_small<MX, OUT, 128>(p, args, w.split, dev, st);
 }
 
 // Argument checks shared by the two products, and the kernel arguments.

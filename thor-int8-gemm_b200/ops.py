@@ -483,11 +483,15 @@ def _fp4_code(kind: str) -> int:
 
 
 def fp4_scale_bytes(rows: int, D: int, kind: str) -> int:
-    """Bytes of the block scales of a [rows, D] 4-bit matrix."""
-    n = _lib.load().t8g_fp4_scale_bytes(rows, D, _fp4_code(kind))
-    if n < 0:
+    """Bytes of the block scales of a [rows, D] 4-bit matrix (as t8g_fp4_scale_bytes)."""
+    _fp4_code(kind)
+    if rows < 0 or D < 0:
         raise ValueError(f"bad sizes {rows} x {D}")
-    return n
+    return _fp4_scale_bytes(rows, D, kind)
+
+
+def _fp4_scale_bytes(rows: int, D: int, kind: str) -> int:
+    return (rows + 127) // 128 * ((D + 127) // 128 if kind == "mxfp4" else (D + 63) // 64) * 512
 
 
 def fp4_scale_rows(sf: torch.Tensor, rows: int, D: int, kind: str) -> torch.Tensor:
@@ -500,8 +504,11 @@ def fp4_scale_rows(sf: torch.Tensor, rows: int, D: int, kind: str) -> torch.Tens
 
 
 def _fp4_empty(S: int, D: int, kind: str, device):
-    q = torch.empty(S, -(-D // 32) * 16, dtype=torch.uint8, device=device)[:, :D // 2]
-    sf = torch.empty(fp4_scale_bytes(S, D, kind), dtype=torch.uint8, device=device)
+    if D % 32:
+        q = torch.empty(S, -(-D // 32) * 16, dtype=torch.uint8, device=device)[:, :D // 2]
+    else:
+        q = torch.empty(S, D // 2, dtype=torch.uint8, device=device)
+    sf = torch.empty(_fp4_scale_bytes(S, D, kind), dtype=torch.uint8, device=device)
     q_scale = torch.empty(S, dtype=torch.float32, device=device) if kind == "nvfp4" else None
     return q, sf, q_scale
 
@@ -545,10 +552,12 @@ def quant_rows_fp4(x: torch.Tensor, kind: str = "nvfp4", stream=None):
     S, D = x.shape
     _fp4_row_len("x", D)
     q, sf, q_scale = _fp4_empty(S, D, kind, x.device)
-    with _on(x.device):
-        rc = _lib.load().t8g_quant_rows_fp4(_ptr(x), _pitch(x, 8), _ptr(q), _pitch(q, 16), _ptr(sf), _ptr(q_scale), S, D,
-                                            code, _stream_handle(x.device, stream))
-    _lib.check(rc)
+    idx = x.get_device()
+    with _on(idx):
+        rc = _lib.load().t8g_quant_rows_fp4(x.data_ptr(), _pitch(x, 8), q.data_ptr(), _pitch(q, 16), sf.data_ptr(),
+                                            _ptr(q_scale), S, D, code, _stream_handle(idx, stream))
+    if rc:
+        _lib.check(rc)
     return q, sf, q_scale
 
 
@@ -631,7 +640,32 @@ def swiglu_quant_fp4_fc1(y: torch.Tensor, kind: str = "nvfp4", stream=None):
 
 
 def _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype):
-    """Argument rules of the 4-bit products -> (M, N, K, w_scale numel, bias numel)."""
+    """Argument rules of the 4-bit products -> (M, N, K, w_scale numel, bias numel).  The common case
+    is checked cheaply, all tensors on one device; anything else goes to _fp4_product_explain,
+    which raises the precise error or accepts the call."""
+    try:
+        if x.dtype is torch.uint8 and w.dtype is torch.uint8 and x_sf.dtype is torch.uint8 and w_sf.dtype is torch.uint8:
+            M, Kb = x.shape
+            N, Kw = w.shape
+            K = 2 * Kb
+            d = x.get_device()
+            if (d >= 0 and Kw == Kb and K and not K % 8 and M and N and x.stride(1) == 1 and w.stride(1) == 1
+                    and w.get_device() == d and x_sf.get_device() == d and w_sf.get_device() == d
+                    and x_sf.dim() == 1 and w_sf.dim() == 1 and x_sf.stride(0) == 1 and w_sf.stride(0) == 1
+                    and x_sf.shape[0] >= _fp4_scale_bytes(M, K, kind) and w_sf.shape[0] >= _fp4_scale_bytes(N, K, kind)
+                    and _vector_ok(x_scale, torch.float32, (M,), d) and _vector_ok(w_scale, torch.float32, (1, N), d)
+                    and _vector_ok(bias, out_dtype, (0, N), d)):
+                return M, N, K, 0 if w_scale is None else w_scale.numel(), 0 if bias is None else bias.numel()
+    except (AttributeError, TypeError, ValueError, IndexError):
+        pass
+    return _fp4_product_explain(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype)
+
+
+def _vector_ok(t, dtype, sizes, device) -> bool:
+    return t is None or (t.dtype is dtype and t.numel() in sizes and t.is_contiguous() and t.get_device() == device)
+
+
+def _fp4_product_explain(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype):
     M, K = _fp4_operand("x", x, x_sf, kind)
     N, Kw = _fp4_operand("w", w, w_sf, kind)
     if Kw != K:
@@ -651,12 +685,15 @@ def _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype)
         _need_cuda("bias", bias, out_dtype)
         if nb != N or not bias.is_contiguous():
             raise ValueError("bias must be contiguous with N elements, in the output dtype")
+    _one_device(x=x, w=w, x_sf=x_sf, w_sf=w_sf, x_scale=x_scale, w_scale=w_scale, bias=bias if nb else None)
     return M, N, K, 0 if w_scale is None else w_scale.numel(), nb
 
 
 def _out_matrix(M: int, N: int, dtype: torch.dtype, device) -> torch.Tensor:
     """[M, N] with rows at a multiple of 16 bytes (contiguous when N allows)."""
     per = 16 // dtype.itemsize
+    if N % per == 0:
+        return torch.empty(M, N, dtype=dtype, device=device)
     return torch.empty(M, -(-N // per) * per, dtype=dtype, device=device)[:, :N]
 
 
@@ -678,16 +715,19 @@ def gemm_fp4(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: torch.T
     M, N, K, nws, nb = _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype)
     if out is None:
         out = _out_matrix(M, N, out_dtype, x.device)
-    _need_cuda("out", out, out_dtype, 2)
-    if tuple(out.shape) != (M, N):
-        raise ValueError(f"out has shape {tuple(out.shape)}, expected {(M, N)}")
-    _one_device(x=x, w=w, x_sf=x_sf, w_sf=w_sf, x_scale=x_scale, w_scale=w_scale, bias=bias if nb else None, out=out)
-    with _on(x.device):
+    else:
+        _need_cuda("out", out, out_dtype, 2)
+        if tuple(out.shape) != (M, N):
+            raise ValueError(f"out has shape {tuple(out.shape)}, expected {(M, N)}")
+        _one_device(x=x, out=out)
+    idx = x.get_device()
+    with _on(idx):
         rc = _lib.load().t8g_gemm_fp4(
-            _ptr(x), _ptr(x_sf), _ptr(x_scale), _ptr(w), _ptr(w_sf), _ptr(w_scale), nws, _ptr(bias) if nb else None, nb,
-            _ptr(out), OUT_CODE[out_dtype], M, N, K, _pitch(x, 16), _pitch(w, 16), _pitch(out, 16 // out_dtype.itemsize),
-            code, _stream_handle(x.device, stream))
-    _lib.check(rc)
+            x.data_ptr(), x_sf.data_ptr(), _ptr(x_scale), w.data_ptr(), w_sf.data_ptr(), _ptr(w_scale), nws,
+            bias.data_ptr() if nb else None, nb, out.data_ptr(), OUT_CODE[out_dtype], M, N, K, _pitch(x, 16),
+            _pitch(w, 16), _pitch(out, 16 // out_dtype.itemsize), code, _stream_handle(idx, stream))
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -724,17 +764,22 @@ def gemm_fp4_gated(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: t
             raise ValueError(f"rows_per_gate={rpg} maps rows past the {gate.shape[0]} gate rows")
     if out is None:
         out = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
-    _need_cuda("out", out, torch.bfloat16, 2)
-    if tuple(out.shape) != (M, N):
-        raise ValueError(f"out has shape {tuple(out.shape)}, expected {(M, N)}")
-    _one_device(x=x, w=w, x_sf=x_sf, w_sf=w_sf, x_scale=x_scale, w_scale=w_scale, bias=bias if nb else None, res=res,
-                gate=gate, gate_index=gate_index, out=out)
-    with _on(x.device):
+    elif out is not res:
+        _need_cuda("out", out, torch.bfloat16, 2)
+        if tuple(out.shape) != (M, N):
+            raise ValueError(f"out has shape {tuple(out.shape)}, expected {(M, N)}")
+    idx = x.get_device()
+    if (res.get_device() != idx or gate.get_device() != idx or out.get_device() != idx
+            or (gate_index is not None and gate_index.get_device() != idx)):
+        _one_device(x=x, res=res, gate=gate, gate_index=gate_index, out=out)
+    with _on(idx):
         rc = _lib.load().t8g_gemm_fp4_gated(
-            _ptr(x), _ptr(x_sf), _ptr(x_scale), _ptr(w), _ptr(w_sf), _ptr(w_scale), nws, _ptr(bias) if nb else None, nb,
-            _ptr(res), _pitch(res, 8), _ptr(gate), _pitch(gate, 8), _ptr(gate_index), rpg, _ptr(out), M, N, K,
-            _pitch(x, 16), _pitch(w, 16), _pitch(out, 8), code, _stream_handle(x.device, stream))
-    _lib.check(rc)
+            x.data_ptr(), x_sf.data_ptr(), _ptr(x_scale), w.data_ptr(), w_sf.data_ptr(), _ptr(w_scale), nws,
+            bias.data_ptr() if nb else None, nb, res.data_ptr(), _pitch(res, 8), gate.data_ptr(), _pitch(gate, 8),
+            _ptr(gate_index), rpg, out.data_ptr(), M, N, K, _pitch(x, 16), _pitch(w, 16), _pitch(out, 8), code,
+            _stream_handle(idx, stream))
+    if rc:
+        _lib.check(rc)
     return out
 
 

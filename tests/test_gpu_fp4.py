@@ -33,14 +33,13 @@ def check_operand(got, x, kind):
     # a zero may carry either sign; what stands under a NaN scale is not looked at
     same = (gcode == code) | (((gcode | code) & 7) == 0) | dead
     assert same.all(), np.argwhere(~same)[:5]
-    gsf = sf.cpu().numpy()
-    assert gsf.size == ops.fp4_scale_bytes(S, D, kind)
-    ref = F4.tile_scales(byte)
-    if kind == "nvfp4" and np.isnan(rs).any():
-        rows = ops.fp4_scale_rows(sf, S, D, kind).cpu().numpy()
-        assert np.array_equal(rows[~np.isnan(rs)], byte[~np.isnan(rs)])
-    else:
-        assert np.array_equal(gsf, ref)
+    assert sf.numel() == ops.fp4_scale_bytes(S, D, kind)
+    # rows of the tiles, blocks filled up to a multiple of four with zeros
+    words = F4.tile_scales(byte).reshape(-(-S // 128), -1, 32, 4, 4).transpose(0, 3, 2, 1, 4).reshape(-(-S // 128) * 128, -1)[:S]
+    got_words = sf.cpu().numpy().reshape(-(-S // 128), -1, 32, 4, 4).transpose(0, 3, 2, 1, 4).reshape(-(-S // 128) * 128, -1)[:S]
+    ok = np.ones(S, bool) if rs is None else ~np.isnan(rs)
+    assert np.array_equal(got_words[ok], words[ok])
+    assert np.array_equal(ops.fp4_scale_rows(sf, S, D, kind).cpu().numpy()[ok], byte[ok])
 
 
 @pytest.mark.parametrize("kind", KINDS)

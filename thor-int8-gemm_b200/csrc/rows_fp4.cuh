@@ -16,8 +16,9 @@
 // A block with a NaN or an infinity has a NaN scale; a row with one has (nvfp4) a NaN row scale,
 // so every product with that row is NaN.
 //
-// Scales are stored in tiles of 128 rows x 4 blocks (gemm_fp4.cuh); rows past the last one, up to a
-// multiple of 128, and blocks past the last one, up to a multiple of 4, are written as 0.
+// Scales are stored in tiles of 128 rows x 4 blocks (gemm_fp4.cuh).  Blocks past a row's last one, up to a
+// multiple of 4, are written as 0 (their codes are read as 0, and 0 times a NaN scale would not
+// be); rows past the last one are left as they were (they reach no output that is stored).
 #pragma once
 
 #include "rows.cuh"
@@ -148,39 +149,18 @@ __device__ __forceinline__ void store_vec_fp4(const Fp4Out& o, uint8_t* qrow, ui
   }
 }
 
-// Scale words of the rows that fill up the last tile: zeros, dealt over the grid's warps.
-__device__ __forceinline__ void zero_pad_rows(const Fp4Out& o) {
-  const int64_t end = (o.S + 127) & ~static_cast<int64_t>(127);
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
-  for (int64_t row = o.S + static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); row < end;
-       row += warps)
-    for (int w = threadIdx.x & 31; w < o.words; w += 32)
-      *reinterpret_cast<uint32_t*>(o.sf + scale_row(row, o.words) + 512 * static_cast<int64_t>(w)) = 0u;
-}
-
-// ---------------------------------------------------------------- quantisation
-// One row per warp (rows of at most kWarpRowMaxBytes).
-template <bool MX>
-__global__ void __launch_bounds__(1024) quant_rows_fp4_warp_kernel(const QuantRowsArgs a, const WarpRingGeom g,
-                                                                   const Fp4Out o) {
-  extern __shared__ __align__(1024) uint8_t smem[];
-  const int lane = threadIdx.x & 31;
-  const int nvec = a.D >> 3;
-  auto src = [&](int64_t r) -> const void* { return a.x + r * a.ld_x; };
-  warp_row_loop(smem, g, a.S, src, [&](int64_t row, const uint8_t* slot) {
-    float inverse = 0.f;
-    if constexpr (!MX) {
-      uint32_t m = 0;
-      for (int c = lane; c < nvec; c += 32) m = max(m, absmax_bits(lds_v4(slot + 16 * c)));
-      const float scale = row_scale_fp4(warp_max_u32(m), &inverse);
-      if (lane == 0) o.q_scale[row] = scale;
-    }
-    uint8_t* qrow = o.q + row * o.ld_q;
-    uint8_t* sfrow = o.sf + scale_row(row, o.words);
-    for (int c = lane; c - lane < nvec; c += 32)
-      store_vec_fp4<MX>(o, qrow, sfrow, c, nvec, c < nvec ? lds_v4(slot + 16 * c) : make_uint4(0, 0, 0, 0), inverse);
-  });
-  zero_pad_rows(o);
+// ---------------------------------------------------------------- direct row kernels
+// Quantisation and norm: a row group of T threads per row with its V vectors a thread in registers
+// (thread t holds vectors t, t + T, ...), loaded straight from global memory; a CTA holds as many
+// groups as make 256 threads and runs once.  Enough CTAs share an SM to keep 50 KB and more of
+// loads in flight, so no ring is needed, and a single row takes one round trip.  (T, V) is the
+// canonical row-group shape, which makes the norm's sum of squares the 8-bit kernels', bit for bit.
+__device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
 }
 
 // Row maximum (bf16 bits) over a row group.
@@ -193,120 +173,85 @@ __device__ __forceinline__ uint32_t group_max_u32(const RowGroup& grp, uint32_t 
   return warp_max_u32(lane < (grp.T >> 5) ? __float_as_uint(red[lane]) : 0u);
 }
 
-// The quantising pass of a row group over bf16 vectors in its slot.
-template <bool MX>
-__device__ __forceinline__ void group_quant_fp4(const RowGroup& grp, const Fp4Out& o, int64_t row, const uint8_t* slot,
-                                                int nvec, float inverse) {
+// Quantises the V vectors a thread of the group holds (zeros past the row's end).
+template <bool MX, int V>
+__device__ __forceinline__ void group_quant_fp4(const RowGroup& grp, const Fp4Out& o, int64_t row, const uint4 (&v)[V],
+                                                int nvec, float* red) {
+  float inverse = 0.f;
+  if constexpr (!MX) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) m = max(m, absmax_bits(v[i]));
+    const float scale = row_scale_fp4(group_max_u32(grp, m, red), &inverse);
+    if (grp.t == 0) o.q_scale[row] = scale;
+  }
   uint8_t* qrow = o.q + row * o.ld_q;
   uint8_t* sfrow = o.sf + scale_row(row, o.words);
-  const int lane = grp.t & 31;
-  for (int c = grp.t; c - lane < nvec; c += grp.T)
-    store_vec_fp4<MX>(o, qrow, sfrow, c, nvec, c < nvec ? lds_v4(slot + 16 * c) : make_uint4(0, 0, 0, 0), inverse);
-}
-
-// Longer rows: one CTA per row.
-template <bool MX>
-__global__ void __launch_bounds__(512) quant_rows_fp4_kernel(const QuantRowsArgs a, const RingGeom g, const Fp4Out o) {
-  extern __shared__ __align__(1024) uint8_t smem[];
-  const RowGroup grp = row_group(blockDim.x);
-  const int nvec = a.D >> 3;
-  auto src = [&](int64_t r, int) -> const void* { return a.x + r * a.ld_x; };
-  row_loop(smem, g, grp, a.S, src, [&](int64_t row, const uint8_t* slot, const RingState& rs) {
-    float inverse = 0.f;
-    if constexpr (!MX) {
-      uint32_t m = 0;
-      for (int c = grp.t; c < nvec; c += grp.T) m = max(m, absmax_bits(lds_v4(slot + 16 * c)));
-      const float scale = row_scale_fp4(group_max_u32(grp, m, rs.red_max), &inverse);
-      if (grp.t == 0) o.q_scale[row] = scale;
-    }
-    group_quant_fp4<MX>(grp, o, row, slot, nvec, inverse);
-  });
-  zero_pad_rows(o);
-}
-
-// ---------------------------------------------------------------- RMSNorm + modulation
-// The norm of rms_mod_warp_kernel / rms_mod_kernel (the same sums in the same order: h is bit for
-// bit theirs), bf16(h) left in the slot and quantised from there.
-template <bool MX>
-__global__ void __launch_bounds__(1024) rms_mod_fp4_warp_kernel(const RmsArgs a, const WarpRingGeom g, const Fp4Out o,
-                                                                const int T) {
-  extern __shared__ __align__(1024) uint8_t smem[];
-  const int lane = threadIdx.x & 31;
-  const int nvec = a.D >> 3;
-  const int nw = T >> 5;
-  const float fD = static_cast<float>(a.D);
-  auto src = [&](int64_t r) -> const void* { return a.x + r * a.ld_x; };
-  warp_row_loop(smem, g, a.S, src, [&](int64_t row, uint8_t* slot) {
-    float ss = 0.f;
-    for (int j = 0; j < nw; ++j) {
-      float2 acc = make_float2(0.f, 0.f);
-      for (int c = 32 * j + lane; c < nvec; c += T) acc = row_sumsq_vec(acc, lds_v4(slot + 16 * c));
-      float v = __fadd_rn(acc.x, acc.y);
 #pragma unroll
-      for (int off = 16; off >= 1; off >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xFFFFFFFFu, v, off));
-      ss = j == 0 ? v : __fadd_rn(ss, v);
-    }
-    const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, fD), a.eps)));
-    const int64_t m = a.mod_index ? static_cast<int64_t>(__ldg(a.mod_index + row)) : row / a.rows_per_mod;
-    uint32_t mx = 0;
-    for (int c = lane; c < nvec; c += 32) {
-      float2 s[4], b[4], x[4], h[4];
-      load_mod8(a, m, c, s, b);
-      rms_h8(lds_v4(slot + 16 * c), make_float2(inv, inv), s, b, a.w, c, x, h);
-      const uint4 hu = make_uint4(f2_to_bf2(h[0]), f2_to_bf2(h[1]), f2_to_bf2(h[2]), f2_to_bf2(h[3]));
-      mx = max(mx, absmax_bits(hu));
-      *reinterpret_cast<uint4*>(slot + 16 * c) = hu;
-    }
-    float inverse = 0.f;
-    if constexpr (!MX) {
-      const float scale = row_scale_fp4(warp_max_u32(mx), &inverse);
-      if (lane == 0) o.q_scale[row] = scale;
-    }
-    uint8_t* qrow = o.q + row * o.ld_q;
-    uint8_t* sfrow = o.sf + scale_row(row, o.words);
-    for (int c = lane; c - lane < nvec; c += 32)   // every lane reads back what it wrote
-      store_vec_fp4<MX>(o, qrow, sfrow, c, nvec, c < nvec ? lds_v4(slot + 16 * c) : make_uint4(0, 0, 0, 0), inverse);
-  });
-  zero_pad_rows(o);
+  for (int i = 0; i < V; ++i) {
+    const int c = grp.t + grp.T * i;
+    if (c - (grp.t & 31) < nvec) store_vec_fp4<MX>(o, qrow, sfrow, c, nvec, v[i], inverse);   // warp-uniform
+  }
 }
 
-template <bool MX>
-__global__ void __launch_bounds__(512) rms_mod_fp4_kernel(const RmsArgs a, const RingGeom g, const Fp4Out o) {
-  extern __shared__ __align__(1024) uint8_t smem[];
-  const RowGroup grp = row_group(blockDim.x);
+template <bool MX, int V>
+__global__ void __launch_bounds__(512) quant_rows_fp4_kernel(const QuantRowsArgs a, const Fp4Out o, const int T) {
+  __shared__ float red[16];
+  const RowGroup grp = row_group(T);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * grp.count + grp.index;
   const int nvec = a.D >> 3;
-  const float fD = static_cast<float>(a.D);
-  auto src = [&](int64_t r, int) -> const void* { return a.x + r * a.ld_x; };
-  row_loop(smem, g, grp, a.S, src, [&](int64_t row, uint8_t* slot, const RingState& rs) {
+  if (row < a.S) {
+    const __nv_bfloat16* x = a.x + row * a.ld_x;
+    uint4 v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = grp.t + T * i;
+      v[i] = c < nvec ? ld_stream_v4(x + 8 * c) : make_uint4(0, 0, 0, 0);
+    }
+    group_quant_fp4<MX, V>(grp, o, row, v, nvec, red + grp.index * (T >> 5));
+  }
+}
+
+// RMSNorm + modulation as rms_mod_kernel computes them; only bf16(h)'s quantisation is stored.
+template <bool MX, int V>
+__global__ void __launch_bounds__(512) rms_mod_fp4_kernel(const RmsArgs a, const Fp4Out o, const int T) {
+  __shared__ float red_sum[16], red_max[16];
+  const RowGroup grp = row_group(T);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * grp.count + grp.index;
+  const int nvec = a.D >> 3;
+  if (row < a.S) {
+    const __nv_bfloat16* x = a.x + row * a.ld_x;
+    uint4 v[V];
     float2 acc = make_float2(0.f, 0.f);
-    for (int c = grp.t; c < nvec; c += grp.T) acc = row_sumsq_vec(acc, lds_v4(slot + 16 * c));
-    const float ss = block_sum(grp, __fadd_rn(acc.x, acc.y), rs.red_sum);
-    const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, fD), a.eps)));
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = grp.t + T * i;
+      v[i] = c < nvec ? ld_stream_v4(x + 8 * c) : make_uint4(0, 0, 0, 0);
+    }
     const int64_t m = a.mod_index ? static_cast<int64_t>(__ldg(a.mod_index + row)) : row / a.rows_per_mod;
-    uint32_t mx = 0;
-    for (int c = grp.t; c < nvec; c += grp.T) {
-      float2 s[4], b[4], x[4], h[4];
-      load_mod8(a, m, c, s, b);
-      rms_h8(lds_v4(slot + 16 * c), make_float2(inv, inv), s, b, a.w, c, x, h);
-      const uint4 hu = make_uint4(f2_to_bf2(h[0]), f2_to_bf2(h[1]), f2_to_bf2(h[2]), f2_to_bf2(h[3]));
-      mx = max(mx, absmax_bits(hu));
-      *reinterpret_cast<uint4*>(slot + 16 * c) = hu;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (grp.t + T * i < nvec) acc = row_sumsq_vec(acc, v[i]);
+    const float ss = block_sum(grp, __fadd_rn(acc.x, acc.y), red_sum + grp.index * (T >> 5));
+    const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(a.D)), a.eps)));
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = grp.t + T * i;
+      if (c < nvec) {
+        float2 s[4], b[4], xv[4], h[4];
+        load_mod8(a, m, c, s, b);
+        rms_h8(v[i], make_float2(inv, inv), s, b, a.w, c, xv, h);
+        v[i] = make_uint4(f2_to_bf2(h[0]), f2_to_bf2(h[1]), f2_to_bf2(h[2]), f2_to_bf2(h[3]));
+      }
     }
-    slot_written();
-    float inverse = 0.f;
-    if constexpr (!MX) {
-      const float scale = row_scale_fp4(group_max_u32(grp, mx, rs.red_max), &inverse);
-      if (grp.t == 0) o.q_scale[row] = scale;
-    }
-    group_quant_fp4<MX>(grp, o, row, slot, nvec, inverse);   // every thread reads back what it wrote
-  });
-  zero_pad_rows(o);
+    group_quant_fp4<MX, V>(grp, o, row, v, nvec, red_max + grp.index * (T >> 5));
+  }
 }
 
 // ---------------------------------------------------------------- SwiGLU
-// act = bf16((gate * sigmoid(gate)) * up) as swiglu_kernel computes it, kept in the gate row's
-// slot and quantised from there.
-template <bool MX>
+// act = bf16((gate * sigmoid(gate)) * up) as swiglu_kernel computes it, on its ring (the sigmoid table
+// is worth loading only once per CTA), quantised from registers.
+template <bool MX, int V>
 __global__ void __launch_bounds__(1024) swiglu_fp4_kernel(const SwigluArgs a, const RingGeom g, const Fp4Out o,
                                                           const int T) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -319,27 +264,35 @@ __global__ void __launch_bounds__(1024) swiglu_fp4_kernel(const SwigluArgs a, co
   auto src = [&](int64_t r, int part) -> const void* { return (part ? a.up : a.gate) + r * a.ld_in; };
   row_loop(ring, g, grp, a.M, src, [&](int64_t row, uint8_t* slot, const RingState& rs) {
     const uint8_t* up = slot + g.part_bytes;
-    uint32_t mx = 0;
     float unused = 0.f;
-    for (int c = grp.t; c < nvec; c += T) {
-      const uint4 au = swiglu8(slot, up, c, sig, unused, false);
-      mx = max(mx, absmax_bits(au));
-      *reinterpret_cast<uint4*>(slot + 16 * c) = au;
+    uint4 v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = grp.t + T * i;
+      v[i] = c < nvec ? swiglu8(slot, up, c, sig, unused, false) : make_uint4(0, 0, 0, 0);
     }
-    slot_written();
-    float inverse = 0.f;
-    if constexpr (!MX) {
-      const float scale = row_scale_fp4(group_max_u32(grp, mx, rs.red_max), &inverse);
-      if (grp.t == 0) o.q_scale[row] = scale;
-    }
-    group_quant_fp4<MX>(grp, o, row, slot, nvec, inverse);   // every thread reads back what it wrote
+    group_quant_fp4<MX, V>(grp, o, row, v, nvec, rs.red_max);
   });
-  zero_pad_rows(o);
 }
 
 // ---------------------------------------------------------------- inverse
 // out[m, k] = cast((code * block scale) * row scale), one vector of eight values per thread.
 // OUT: 0 bf16, 1 fp16, 2 fp32.
+// Eight codes -> their e2m1 values.
+__device__ __forceinline__ void decode_e2m1x8(uint32_t codes, float2 (&v)[4]) {
+  uint32_t h[4];
+  asm("{ .reg .b8 a, b, c, d;\n"
+      "  mov.b32 {a, b, c, d}, %4;\n"
+      "  cvt.rn.f16x2.e2m1x2 %0, a;\n"
+      "  cvt.rn.f16x2.e2m1x2 %1, b;\n"
+      "  cvt.rn.f16x2.e2m1x2 %2, c;\n"
+      "  cvt.rn.f16x2.e2m1x2 %3, d; }"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(codes));
+#pragma unroll
+  for (int p = 0; p < 4; ++p) v[p] = __half22float2(*reinterpret_cast<const __half2*>(&h[p]));
+}
+
 struct DequantFp4Args {
   const uint8_t* q;
   int64_t ld_q;
@@ -354,44 +307,51 @@ struct DequantFp4Args {
 
 template <bool MX, int OUT>
 __global__ void __launch_bounds__(256) dequant_rows_fp4_kernel(const DequantFp4Args a) {
+  // thread = one vector of eight; a CTA covers 256 vectors of one row group of rows (gridDim.y strides over rows)
   const int nvec = a.D >> 3;
-  const int64_t total = a.S * nvec;
-  const int64_t G = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += G) {
-    const int64_t row = i / nvec;
-    const int c = static_cast<int>(i - row * nvec);
-    const uint32_t codes = __ldg(reinterpret_cast<const uint32_t*>(a.q + row * a.ld_q + 4 * c));
-    const int block = MX ? c >> 2 : c >> 1;
-    const uint32_t byte = __ldg(a.sf + scale_row(row, a.words) + 512 * static_cast<int64_t>(block >> 2) + (block & 3));
-    const float rs = a.q_scale ? __ldg(a.q_scale + row) : 1.f;
-    const float sb = MX ? __uint_as_float(byte == 255u ? 0x7FC00000u : byte == 0u ? 0x00400000u : byte << 23)
-                        : e4m3_to_f32(byte);
-    float v[8];
+  const int c = blockIdx.x * blockDim.x + threadIdx.x;
+  if (c >= nvec) return;
+  const int block = MX ? c >> 2 : c >> 1;
+  const int64_t sf_at = 512 * static_cast<int64_t>(block >> 2) + (block & 3);
+  constexpr int kRows = 4;   // rows in flight per thread
+  for (int64_t row0 = static_cast<int64_t>(blockIdx.y) * kRows; row0 < a.S; row0 += static_cast<int64_t>(gridDim.y) * kRows) {
+    uint32_t codes[kRows], byte[kRows];
+    float rs[kRows];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      // e2m1: two exponent bits (bias 1), one mantissa bit
-      const uint32_t code = codes >> (4 * j);
-      const uint32_t mag = code & 7u;
-      const float e = mag < 2u ? 0.5f * static_cast<float>(mag)
-                               : __uint_as_float(((126u + (mag >> 1)) << 23) | ((mag & 1u) << 22));
-      v[j] = __fmul_rn(__fmul_rn((code & 8u) ? -e : e, sb), rs);
+    for (int r = 0; r < kRows; ++r) {
+      const int64_t row = min(row0 + r, a.S - 1);
+      codes[r] = __ldg(reinterpret_cast<const uint32_t*>(a.q + row * a.ld_q + 4 * static_cast<int64_t>(c)));
+      byte[r] = __ldg(a.sf + scale_row(row, a.words) + sf_at);
+      rs[r] = a.q_scale ? __ldg(a.q_scale + row) : 1.f;
     }
-    if constexpr (OUT == 2) {
-      float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * a.ld_out + 8 * c);
-      p[0] = make_float4(v[0], v[1], v[2], v[3]);
-      p[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      uint32_t w[4];
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        if constexpr (OUT == 0) {
-          w[p] = pack_bf16(v[2 * p], v[2 * p + 1]);
-        } else {
-          const __half2 h = __floats2half2_rn(v[2 * p], v[2 * p + 1]);
-          w[p] = *reinterpret_cast<const uint32_t*>(&h);
+    for (int r = 0; r < kRows; ++r) {
+      const int64_t row = row0 + r;
+      if (row >= a.S) break;
+      const float sb = MX ? __uint_as_float(byte[r] == 255u ? 0x7FC00000u : byte[r] == 0u ? 0x00400000u : byte[r] << 23)
+                          : e4m3_to_f32(byte[r]);
+      float2 v[4];
+      decode_e2m1x8(codes[r], v);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) v[p] = mul2_rn(mul2_rn(v[p], make_float2(sb, sb)), make_float2(rs[r], rs[r]));
+      const int64_t at = row * a.ld_out + 8 * static_cast<int64_t>(c);
+      if constexpr (OUT == 2) {
+        float4* p = reinterpret_cast<float4*>(static_cast<float*>(a.out) + at);
+        p[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        p[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+      } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          if constexpr (OUT == 0) {
+            w[p] = f2_to_bf2(v[p]);
+          } else {
+            const __half2 h = __floats2half2_rn(v[p].x, v[p].y);
+            w[p] = *reinterpret_cast<const uint32_t*>(&h);
+          }
         }
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at) = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + row * a.ld_out + 8 * c) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }

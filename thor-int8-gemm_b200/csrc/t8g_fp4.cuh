@@ -43,6 +43,36 @@ t8g::rows::Fp4Out fp4_out(void* q, int64_t ld_q, void* sf, float* q_scale, int64
   return o;
 }
 
+// Vectors per thread of a direct row kernel: the canonical shape's, rounded up to a compiled one.
+#define T8G_DISPATCH_FP4_V(v, CALL)                    \
+  if ((v) <= 3) {                                      \
+    constexpr int V = 3;                               \
+    CALL;                                              \
+  } else if ((v) <= 6) {                               \
+    constexpr int V = 6;                               \
+    CALL;                                              \
+  } else {                                             \
+    constexpr int V = 12;                              \
+    CALL;                                              \
+  }
+
+// Launch shape of a direct row kernel: T threads a row, as many rows a CTA as make 256 threads.
+struct Fp4RowsLaunch {
+  int T, V;
+  unsigned grid, threads;
+};
+int fp4_rows_launch(const char* what, int64_t S, int64_t D, Fp4RowsLaunch* l) {
+  const int64_t nvec = D / 8;
+  l->T = row_shape(D).T;
+  l->V = static_cast<int>((nvec + l->T - 1) / l->T);
+  const int groups = l->T <= 128 ? 256 / l->T : 1;
+  const int64_t grid = (S + groups - 1) / groups;
+  if (grid >= (int64_t(1) << 31)) return fail(T8G_ERR_UNSUPPORTED, "%s: too many rows", what);
+  l->grid = static_cast<unsigned>(grid);
+  l->threads = static_cast<unsigned>(groups * l->T);
+  return T8G_OK;
+}
+
 // ----------------------------------------------------------------- GEMM
 struct Fp4Gemm {
   const void *x, *x_sf, *w, *w_sf;
@@ -234,16 +264,14 @@ int t8g_quant_rows_fp4(const void* x, int64_t ld_x, void* q, int64_t ld_q, void*
   a.S = S;
   a.D = static_cast<int>(D);
   const Fp4Out o = fp4_out(q, ld_q, sf, q_scale, S, D, quant_kind);
-  const uint32_t row_bytes = static_cast<uint32_t>(2 * D);
-  const bool mx = quant_kind == T8G_QUANT_MXFP4;
-  if (row_bytes <= kWarpRowMaxBytes)
-    return mx ? launch_warp_rows(quant_rows_fp4_warp_kernel<true>, a, row_bytes, S, dev, info.sms, st, WarpLaunch{},
-                                 "quant_rows_fp4", o)
-              : launch_warp_rows(quant_rows_fp4_warp_kernel<false>, a, row_bytes, S, dev, info.sms, st, WarpLaunch{},
-                                 "quant_rows_fp4", o);
-  const int T = row_shape(D).T;
-  return mx ? launch_rows(quant_rows_fp4_kernel<true>, T, a, ring_geom(D, 1), S, dev, info.sms, st, "quant_rows_fp4", o)
-            : launch_rows(quant_rows_fp4_kernel<false>, T, a, ring_geom(D, 1), S, dev, info.sms, st, "quant_rows_fp4", o);
+  Fp4RowsLaunch l;
+  if ((rc = fp4_rows_launch("quant_rows_fp4", S, D, &l))) return rc;
+  if (quant_kind == T8G_QUANT_MXFP4) {
+    T8G_DISPATCH_FP4_V(l.V, (quant_rows_fp4_kernel<true, V><<<l.grid, l.threads, 0, st>>>(a, o, l.T)))
+  } else {
+    T8G_DISPATCH_FP4_V(l.V, (quant_rows_fp4_kernel<false, V><<<l.grid, l.threads, 0, st>>>(a, o, l.T)))
+  }
+  return launch_checked("quant_rows_fp4 launch");
 }
 
 int t8g_rms_mod_quant_fp4(const void* x, int64_t ld_x, const void* w, const void* shift, const void* scale,
@@ -278,16 +306,14 @@ int t8g_rms_mod_quant_fp4(const void* x, int64_t ld_x, const void* w, const void
   a.S = S;
   a.D = static_cast<int>(D);
   const Fp4Out o = fp4_out(q, ld_q, sf, q_scale, S, D, quant_kind);
-  const uint32_t row_bytes = static_cast<uint32_t>(2 * D);
-  const bool mx = quant_kind == T8G_QUANT_MXFP4;
-  const int T = row_shape(D).T;
-  if (row_bytes <= kWarpRowMaxBytes)
-    return mx ? launch_warp_rows(rms_mod_fp4_warp_kernel<true>, a, row_bytes, S, dev, info.sms, st, WarpLaunch{},
-                                 "rms_mod_quant_fp4", o, T)
-              : launch_warp_rows(rms_mod_fp4_warp_kernel<false>, a, row_bytes, S, dev, info.sms, st, WarpLaunch{},
-                                 "rms_mod_quant_fp4", o, T);
-  return mx ? launch_rows(rms_mod_fp4_kernel<true>, T, a, ring_geom(D, 1), S, dev, info.sms, st, "rms_mod_quant_fp4", o)
-            : launch_rows(rms_mod_fp4_kernel<false>, T, a, ring_geom(D, 1), S, dev, info.sms, st, "rms_mod_quant_fp4", o);
+  Fp4RowsLaunch l;
+  if ((rc = fp4_rows_launch("rms_mod_quant_fp4", S, D, &l))) return rc;
+  if (quant_kind == T8G_QUANT_MXFP4) {
+    T8G_DISPATCH_FP4_V(l.V, (rms_mod_fp4_kernel<true, V><<<l.grid, l.threads, 0, st>>>(a, o, l.T)))
+  } else {
+    T8G_DISPATCH_FP4_V(l.V, (rms_mod_fp4_kernel<false, V><<<l.grid, l.threads, 0, st>>>(a, o, l.T)))
+  }
+  return launch_checked("rms_mod_quant_fp4 launch");
 }
 
 int t8g_swiglu_quant_fp4(const void* gate, const void* up, int64_t ld_in, void* q, int64_t ld_q, void* sf, float* q_scale,
@@ -309,11 +335,11 @@ int t8g_swiglu_quant_fp4(const void* gate, const void* up, int64_t ld_in, void* 
   a.M = M;
   a.F = static_cast<int>(F);
   const Fp4Out o = fp4_out(q, ld_q, sf, q_scale, M, F, quant_kind);
-  const int T = swiglu_shape(F).T;
+  const int T = swiglu_shape(F).T;   // at most three vectors a thread
   const RingGeom g = ring_geom(F, 2);
   return quant_kind == T8G_QUANT_MXFP4
-             ? launch_swiglu(swiglu_fp4_kernel<true>, T, a, g, M, dev, info.sms, st, "swiglu_quant_fp4", o)
-             : launch_swiglu(swiglu_fp4_kernel<false>, T, a, g, M, dev, info.sms, st, "swiglu_quant_fp4", o);
+             ? launch_swiglu(swiglu_fp4_kernel<true, kSwigluVecs>, T, a, g, M, dev, info.sms, st, "swiglu_quant_fp4", o)
+             : launch_swiglu(swiglu_fp4_kernel<false, kSwigluVecs>, T, a, g, M, dev, info.sms, st, "swiglu_quant_fp4", o);
 }
 
 int t8g_dequant_rows_fp4(const void* q, int64_t ld_q, const void* sf, const float* q_scale, void* out, int out_dtype,
@@ -340,7 +366,9 @@ int t8g_dequant_rows_fp4(const void* q, int64_t ld_q, const void* sf, const floa
   a.D = static_cast<int>(D);
   a.words = static_cast<int>(fp4_words(D, quant_kind));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((S * (D / 8) + 255) / 256, int64_t(info.sms) * 8));
+  // 256 vectors of four rows a CTA and step; rows are strided over when there are more than the grid holds
+  const unsigned gx = static_cast<unsigned>((D / 8 + 255) / 256);
+  const dim3 grid(gx, static_cast<unsigned>(std::min<int64_t>((S + 3) / 4, 65535)));
 #define T8G_DEQUANT(MX)                                                                               \
   switch (out_dtype) {                                                                                \
     case T8G_OUT_BF16: dequant_rows_fp4_kernel<MX, 0><<<grid, 256, 0, st>>>(a); break;                \

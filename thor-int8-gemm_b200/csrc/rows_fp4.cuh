@@ -126,7 +126,7 @@ __device__ __forceinline__ uint32_t quant_vec_fp4(const uint4& u, float row_inve
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       const float2 y = fma2_rn(v[p], mult2, make_float2(kGrid, kGrid));
-      v[p] = make_float2(__fadd_rn(y.x, -kGrid), __fadd_rn(y.y, -kGrid));
+      v[p] = add2_rn(y, make_float2(-kGrid, -kGrid));
     }
     word = byte << (8 * ((lane >> 1) & 3));
     word |= __shfl_xor_sync(0xFFFFFFFFu, word, 2);
@@ -151,10 +151,11 @@ __device__ __forceinline__ void store_vec_fp4(const Fp4Out& o, uint8_t* qrow, ui
 
 // ---------------------------------------------------------------- direct row kernels
 // Quantisation and norm: a row group of T threads per row with its V vectors a thread in registers
-// (thread t holds vectors t, t + T, ...), loaded straight from global memory; a CTA holds as many
-// groups as make 256 threads and runs once.  Enough CTAs share an SM to keep 50 KB and more of
-// loads in flight, so no ring is needed, and a single row takes one round trip.  (T, V) is the
-// canonical row-group shape, which makes the norm's sum of squares the 8-bit kernels', bit for bit.
+// (thread t holds vectors t, t + T, ...), loaded straight from global memory while the row before is
+// worked on; a CTA holds as many groups as make 256 threads.  A group owns consecutive rows, so it
+// keeps the modulation in registers until the batch element changes.  No ring and no set-up: a
+// single row takes one round trip to memory.  (T, V) is the canonical row-group shape, which makes
+// the norm's sum of squares the 8-bit kernels', bit for bit.
 __device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -194,57 +195,102 @@ __device__ __forceinline__ void group_quant_fp4(const RowGroup& grp, const Fp4Ou
   }
 }
 
-template <bool MX, int V>
-__global__ void __launch_bounds__(512) quant_rows_fp4_kernel(const QuantRowsArgs a, const Fp4Out o, const int T) {
-  __shared__ float red[16];
-  const RowGroup grp = row_group(T);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * grp.count + grp.index;
-  const int nvec = a.D >> 3;
-  if (row < a.S) {
-    const __nv_bfloat16* x = a.x + row * a.ld_x;
-    uint4 v[V];
+template <int V>
+__device__ __forceinline__ void load_row_fp4(uint4 (&v)[V], const __nv_bfloat16* x, int t, int T, int nvec) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = grp.t + T * i;
-      v[i] = c < nvec ? ld_stream_v4(x + 8 * c) : make_uint4(0, 0, 0, 0);
-    }
-    group_quant_fp4<MX, V>(grp, o, row, v, nvec, red + grp.index * (T >> 5));
+  for (int i = 0; i < V; ++i) {
+    const int c = t + T * i;
+    v[i] = c < nvec ? ld_stream_v4(x + 8 * c) : make_uint4(0, 0, 0, 0);
   }
 }
 
-// RMSNorm + modulation as rms_mod_kernel computes them; only bf16(h)'s quantisation is stored.
-template <bool MX, int V>
-__global__ void __launch_bounds__(512) rms_mod_fp4_kernel(const RmsArgs a, const Fp4Out o, const int T) {
-  __shared__ float red_sum[16], red_max[16];
+enum Fp4Source : int { kFp4Plain = 0, kFp4Norm = 1, kFp4NormWeight = 2 };
+
+// rows_per_group rows for each group; a holds x (and, for the norm, its operands).
+template <bool MX, int V, int SRC>
+__global__ void __launch_bounds__(512) rows_fp4_kernel(const RmsArgs a, const Fp4Out o, const int T,
+                                                       const int64_t rows_per_group) {
+  // two of each, used by rows in turn: a warp may write the next row's partials while another still
+  // reads this row's, and the next row's barrier lies between this row's reads and the one after's writes
+  __shared__ float red_sum[2][16], red_max[2][16];
   const RowGroup grp = row_group(T);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * grp.count + grp.index;
+  int turn = 0;
   const int nvec = a.D >> 3;
-  if (row < a.S) {
-    const __nv_bfloat16* x = a.x + row * a.ld_x;
-    uint4 v[V];
-    float2 acc = make_float2(0.f, 0.f);
+  const float fD = static_cast<float>(a.D);
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * grp.count + grp.index) * rows_per_group;
+  const int64_t end = min(first + rows_per_group, a.S);
+  if (first >= end) return;   // a whole group leaves: its barriers are its own
+  uint4 v[V], next[V];
+  load_row_fp4<V>(v, a.x + first * a.ld_x, grp.t, T, nvec);
+  [[maybe_unused]] uint4 mul[SRC ? V : 1], shift[SRC ? V : 1], weight[SRC == kFp4NormWeight ? V : 1];
+  [[maybe_unused]] int64_t cur = -1, seg_end = -1;
+  if constexpr (SRC == kFp4NormWeight) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int c = grp.t + T * i;
-      v[i] = c < nvec ? ld_stream_v4(x + 8 * c) : make_uint4(0, 0, 0, 0);
+      weight[i] = c < nvec ? ld_v4(a.w + 8 * c) : make_uint4(0, 0, 0, 0);
     }
-    const int64_t m = a.mod_index ? static_cast<int64_t>(__ldg(a.mod_index + row)) : row / a.rows_per_mod;
+  }
+  for (int64_t row = first; row < end; ++row) {
+    if (row + 1 < end) load_row_fp4<V>(next, a.x + (row + 1) * a.ld_x, grp.t, T, nvec);
+    if constexpr (SRC != kFp4Plain) {
+      int64_t m = cur;
+      if (a.mod_index) {
+        m = static_cast<int64_t>(__ldg(a.mod_index + row));
+      } else if (row >= seg_end) {
+        m = row / a.rows_per_mod;
+        seg_end = (m + 1) * a.rows_per_mod;
+      }
+      if (m != cur) {   // the same for the whole group
+        cur = m;
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (grp.t + T * i < nvec) acc = row_sumsq_vec(acc, v[i]);
-    const float ss = block_sum(grp, __fadd_rn(acc.x, acc.y), red_sum + grp.index * (T >> 5));
-    const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(a.D)), a.eps)));
+        for (int i = 0; i < V; ++i) {
+          const int c = grp.t + T * i;
+          mul[i] = shift[i] = make_uint4(0, 0, 0, 0);
+          if (c < nvec) {
+            mul[i] = ld_v4(a.scale + m * a.ld_mod + 8 * c);
+            shift[i] = ld_v4(a.shift + m * a.ld_mod + 8 * c);
+          }
+          if (!a.scale_is_multiplier)
+            mul[i] = make_uint4(one_plus_bf16x2(mul[i].x), one_plus_bf16x2(mul[i].y), one_plus_bf16x2(mul[i].z),
+                                one_plus_bf16x2(mul[i].w));
+        }
+      }
+      // vectors past the row's end are zeros and leave the sums as they are
+      float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = grp.t + T * i;
-      if (c < nvec) {
-        float2 s[4], b[4], xv[4], h[4];
-        load_mod8(a, m, c, s, b);
-        rms_h8(v[i], make_float2(inv, inv), s, b, a.w, c, xv, h);
-        v[i] = make_uint4(f2_to_bf2(h[0]), f2_to_bf2(h[1]), f2_to_bf2(h[2]), f2_to_bf2(h[3]));
+      for (int i = 0; i < V; ++i) {
+        acc = sumsq_bf16x2(acc, v[i].x);
+        acc = sumsq_bf16x2(acc, v[i].y);
+        acc = sumsq_bf16x2(acc, v[i].z);
+        acc = sumsq_bf16x2(acc, v[i].w);
+      }
+      const float ss = block_sum(grp, __fadd_rn(acc.x, acc.y), red_sum[turn] + grp.index * (T >> 5));
+      const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, fD), a.eps)));
+      const float2 inv2 = make_float2(inv, inv);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const uint32_t xw[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        const uint32_t sw[4] = {mul[i].x, mul[i].y, mul[i].z, mul[i].w};
+        const uint32_t bw[4] = {shift[i].x, shift[i].y, shift[i].z, shift[i].w};
+        uint32_t h[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          float2 t = mul2_rn(bf2_to_f2(xw[p]), inv2);
+          if constexpr (SRC == kFp4NormWeight) {
+            const uint32_t ww[4] = {weight[i].x, weight[i].y, weight[i].z, weight[i].w};
+            t = mul2_rn(t, bf2_to_f2(ww[p]));
+          }
+          h[p] = f2_to_bf2(add_f32_bf16x2(mul2_rn(t, bf2_to_f2(sw[p])), bw[p]));
+        }
+        v[i] = make_uint4(h[0], h[1], h[2], h[3]);
+        if (grp.t + T * i >= nvec) v[i] = make_uint4(0, 0, 0, 0);   // 0 times an infinite inv
       }
     }
-    group_quant_fp4<MX, V>(grp, o, row, v, nvec, red_max + grp.index * (T >> 5));
+    group_quant_fp4<MX, V>(grp, o, row, v, nvec, red_max[turn] + grp.index * (T >> 5));
+    turn ^= 1;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = next[i];
   }
 }
 

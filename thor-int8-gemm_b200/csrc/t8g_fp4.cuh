@@ -44,33 +44,46 @@ t8g::rows::Fp4Out fp4_out(void* q, int64_t ld_q, void* sf, float* q_scale, int64
 }
 
 // Vectors per thread of a direct row kernel: the canonical shape's, rounded up to a compiled one.
-#define T8G_DISPATCH_FP4_V(v, CALL)                    \
+#define T8G_DISPATCH_FP4_V(v, ...)                     \
   if ((v) <= 3) {                                      \
     constexpr int V = 3;                               \
-    CALL;                                              \
+    __VA_ARGS__;                                       \
   } else if ((v) <= 6) {                               \
     constexpr int V = 6;                               \
-    CALL;                                              \
+    __VA_ARGS__;                                       \
   } else {                                             \
     constexpr int V = 12;                              \
-    CALL;                                              \
+    __VA_ARGS__;                                       \
   }
 
-// Launch shape of a direct row kernel: T threads a row, as many rows a CTA as make 256 threads.
-struct Fp4RowsLaunch {
-  int T, V;
-  unsigned grid, threads;
-};
-int fp4_rows_launch(const char* what, int64_t S, int64_t D, Fp4RowsLaunch* l) {
-  const int64_t nvec = D / 8;
-  l->T = row_shape(D).T;
-  l->V = static_cast<int>((nvec + l->T - 1) / l->T);
-  const int groups = l->T <= 128 ? 256 / l->T : 1;
-  const int64_t grid = (S + groups - 1) / groups;
-  if (grid >= (int64_t(1) << 31)) return fail(T8G_ERR_UNSUPPORTED, "%s: too many rows", what);
-  l->grid = static_cast<unsigned>(grid);
-  l->threads = static_cast<unsigned>(groups * l->T);
+// Launch a direct row kernel: T threads a row, as many rows a CTA as make 256 threads, and no more CTAs
+// than the device holds at a time (each group then takes several consecutive rows).
+template <typename K>
+int launch_rows_fp4(K kern, const t8g::rows::RmsArgs& a, const t8g::rows::Fp4Out& o, int T, int sms, cudaStream_t st,
+                    const char* what) {
+  const int groups = T <= 128 ? 256 / T : 1;
+  const int threads = groups * T;
+  int occ = 0;
+  T8G_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, threads, 0), "occupancy query");
+  const int64_t held = static_cast<int64_t>(occ < 1 ? 1 : occ) * sms * groups;   // rows in work at a time
+  const int64_t per_group = (a.S + held - 1) / held;
+  const int64_t grid = (a.S + per_group * groups - 1) / (per_group * groups);
+  kern<<<static_cast<unsigned>(grid), threads, 0, st>>>(a, o, T, per_group);
+  T8G_CHECK_CUDA(cudaGetLastError(), what);
   return T8G_OK;
+}
+
+template <int SRC>
+int dispatch_rows_fp4(const t8g::rows::RmsArgs& a, const t8g::rows::Fp4Out& o, int quant_kind, int sms, cudaStream_t st,
+                      const char* what) {
+  using namespace t8g::rows;
+  const int T = row_shape(a.D).T;
+  const int v = (a.D / 8 + T - 1) / T;
+  if (quant_kind == T8G_QUANT_MXFP4) {
+    T8G_DISPATCH_FP4_V(v, return launch_rows_fp4(rows_fp4_kernel<true, V, SRC>, a, o, T, sms, st, what))
+  } else {
+    T8G_DISPATCH_FP4_V(v, return launch_rows_fp4(rows_fp4_kernel<false, V, SRC>, a, o, T, sms, st, what))
+  }
 }
 
 // ----------------------------------------------------------------- GEMM
@@ -258,20 +271,13 @@ int t8g_quant_rows_fp4(const void* x, int64_t ld_x, void* q, int64_t ld_q, void*
   DeviceInfo info;
   if ((rc = current_device(&dev, &info))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  QuantRowsArgs a = {};
+  RmsArgs a = {};
   a.x = static_cast<const __nv_bfloat16*>(x);
   a.ld_x = ld_x;
   a.S = S;
   a.D = static_cast<int>(D);
-  const Fp4Out o = fp4_out(q, ld_q, sf, q_scale, S, D, quant_kind);
-  Fp4RowsLaunch l;
-  if ((rc = fp4_rows_launch("quant_rows_fp4", S, D, &l))) return rc;
-  if (quant_kind == T8G_QUANT_MXFP4) {
-    T8G_DISPATCH_FP4_V(l.V, (quant_rows_fp4_kernel<true, V><<<l.grid, l.threads, 0, st>>>(a, o, l.T)))
-  } else {
-    T8G_DISPATCH_FP4_V(l.V, (quant_rows_fp4_kernel<false, V><<<l.grid, l.threads, 0, st>>>(a, o, l.T)))
-  }
-  return launch_checked("quant_rows_fp4 launch");
+  return dispatch_rows_fp4<kFp4Plain>(a, fp4_out(q, ld_q, sf, q_scale, S, D, quant_kind), quant_kind, info.sms, st,
+                                      "quant_rows_fp4");
 }
 
 int t8g_rms_mod_quant_fp4(const void* x, int64_t ld_x, const void* w, const void* shift, const void* scale,
@@ -306,14 +312,8 @@ int t8g_rms_mod_quant_fp4(const void* x, int64_t ld_x, const void* w, const void
   a.S = S;
   a.D = static_cast<int>(D);
   const Fp4Out o = fp4_out(q, ld_q, sf, q_scale, S, D, quant_kind);
-  Fp4RowsLaunch l;
-  if ((rc = fp4_rows_launch("rms_mod_quant_fp4", S, D, &l))) return rc;
-  if (quant_kind == T8G_QUANT_MXFP4) {
-    T8G_DISPATCH_FP4_V(l.V, (rms_mod_fp4_kernel<true, V><<<l.grid, l.threads, 0, st>>>(a, o, l.T)))
-  } else {
-    T8G_DISPATCH_FP4_V(l.V, (rms_mod_fp4_kernel<false, V><<<l.grid, l.threads, 0, st>>>(a, o, l.T)))
-  }
-  return launch_checked("rms_mod_quant_fp4 launch");
+  return w ? dispatch_rows_fp4<kFp4NormWeight>(a, o, quant_kind, info.sms, st, "rms_mod_quant_fp4")
+           : dispatch_rows_fp4<kFp4Norm>(a, o, quant_kind, info.sms, st, "rms_mod_quant_fp4");
 }
 
 int t8g_swiglu_quant_fp4(const void* gate, const void* up, int64_t ld_in, void* q, int64_t ld_q, void* sf, float* q_scale,

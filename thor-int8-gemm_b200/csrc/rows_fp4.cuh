@@ -40,8 +40,20 @@ __host__ __device__ __forceinline__ int64_t scale_row(int64_t row, int words) {
   return (row >> 7) * words * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4;
 }
 
-// Largest magnitude of eight bf16 values as bf16 bits (integer order: NaN above infinity above
-// every number).
+// max(|a|, |b|, |c|), NaN if any of them is.
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)), "f"(fabsf(c)));
+  return d;
+}
+// Largest magnitude of eight values; NaN if one is NaN.
+__device__ __forceinline__ float absmax8(const float2 (&v)[4]) {
+  const float a = max3_abs_nan(v[0].x, v[0].y, v[1].x);
+  const float b = max3_abs_nan(v[1].y, v[2].x, v[2].y);
+  return max3_abs_nan(max3_abs_nan(a, b, v[3].x), v[3].y, 0.f);
+}
+// The same of eight packed bf16 values, as bf16 bits (integer order: NaN above infinity above every
+// number).
 __device__ __forceinline__ uint32_t absmax_bits(const uint4& u) {
   const uint32_t m = max_u16x2(max_u16x2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu),
                                max_u16x2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
@@ -90,35 +102,31 @@ __device__ __forceinline__ float rcp_approx(float v) {   // within 1 ulp; see th
   return r;
 }
 
-// One warp step: lane l holds vector c0 + l of a row (zeros past the row's end).  Returns the
-// eight codes and, in `word`, the four block scales of the lane's group of 16 (mxfp4) or 8
-// (nvfp4) lanes.  Every lane of the warp takes part.
+// One warp step: lane l holds vector c0 + l of a row (zeros past the row's end).  Returns the eight
+// codes and, in `byte`, the scale of the block that the lane's vector lies in (4 lanes a block for
+// mxfp4, 2 for nvfp4).  Every lane of the warp takes part.
 template <bool MX>
-__device__ __forceinline__ uint32_t quant_vec_fp4(const uint4& u, float row_inverse, uint32_t& word) {
-  const int lane = threadIdx.x & 31;
-  uint32_t b = absmax_bits(u);
-  b = max(b, __shfl_xor_sync(0xFFFFFFFFu, b, 1));
-  uint32_t byte;
+__device__ __forceinline__ uint32_t quant_vec_fp4(const uint4& u, float row_inverse, uint32_t& byte) {
   float2 v[4];
   unpack_pairs(u, v);
+  // magnitudes compare as their bits, NaN above all
+  uint32_t b = __float_as_uint(absmax8(v));
+  b = max(b, __shfl_xor_sync(0xFFFFFFFFu, b, 1));
   if constexpr (MX) {
     b = max(b, __shfl_xor_sync(0xFFFFFFFFu, b, 2));
-    const int e = max(static_cast<int>(b >> 7) - 2, 0);
-    const bool finite = b < 0x7F80u;
+    const int e = max(static_cast<int>(b >> 23) - 2, 0);
+    const bool finite = b < 0x7F800000u;
     byte = finite ? static_cast<uint32_t>(e) : 255u;
     const float mult = finite ? __uint_as_float(static_cast<uint32_t>(254 - e) << 23) : 0.f;
 #pragma unroll
     for (int p = 0; p < 4; ++p) v[p] = mul2_rn(v[p], make_float2(mult, mult));
-    word = byte << (8 * ((lane >> 2) & 3));
-    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
-    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 8);
   } else {
     // RN(t / 6) with one correction step (quant8 of rows.cuh), then e4m3
-    const float t = __fmul_rn(__uint_as_float(b << 16), row_inverse);
+    const float t = __fmul_rn(__uint_as_float(b), row_inverse);
     const float sixth = 1.0f / 6.0f;
     const float q0 = __fmul_rn(t, sixth);
     const float q1 = __fmaf_rn(__fmaf_rn(-6.0f, q0, t), sixth, q0);
-    byte = cvt_e4m3x2(q1, 0.f) & 0xFFu;
+    byte = cvt_e4m3x2(q1, 0.f);
     const float sb = e4m3_to_f32(byte);
     const float mult = sb > 0.f ? __fmul_rn(row_inverse, rcp_approx(sb)) : 0.f;
     const float2 mult2 = make_float2(mult, mult);
@@ -128,25 +136,22 @@ __device__ __forceinline__ uint32_t quant_vec_fp4(const uint4& u, float row_inve
       const float2 y = fma2_rn(v[p], mult2, make_float2(kGrid, kGrid));
       v[p] = add2_rn(y, make_float2(-kGrid, -kGrid));
     }
-    word = byte << (8 * ((lane >> 1) & 3));
-    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 2);
-    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 4);
   }
   return cvt_e2m1x8(v);
 }
 
-// Vectors c0 + lane (a multiple of 32 apart) of row `row`, held in u: codes and scale words.
+// Vector c of a row, held in u by lane c % 32 (vectors of a warp step are consecutive): its codes,
+// and its block's scale from the block's first lane.
 template <bool MX>
-__device__ __forceinline__ void store_vec_fp4(const Fp4Out& o, uint8_t* qrow, uint8_t* sfrow, int c, int nvec,
-                                              const uint4& u, float row_inverse) {
-  constexpr int kLanesPerWord = MX ? 16 : 8;
-  uint32_t word;
-  const uint32_t codes = quant_vec_fp4<MX>(u, row_inverse, word);
-  if (c < nvec) {
-    *reinterpret_cast<uint32_t*>(qrow + 4 * c) = codes;
-    if ((c & (kLanesPerWord - 1)) == 0)
-      *reinterpret_cast<uint32_t*>(sfrow + 512 * static_cast<int64_t>(c / kLanesPerWord)) = word;
-  }
+__device__ __forceinline__ void store_vec_fp4(uint8_t* qrow, uint8_t* sfrow, int c, int nvec, const uint4& u,
+                                              float row_inverse) {
+  constexpr int kLanes = MX ? 4 : 2;   // per block
+  uint32_t byte;
+  const uint32_t codes = quant_vec_fp4<MX>(u, row_inverse, byte);
+  if (c < nvec) *reinterpret_cast<uint32_t*>(qrow + 4 * c) = codes;
+  // blocks past the row's last, up to a multiple of four, get the 0 that vectors of zeros have
+  if ((c & (kLanes - 1)) == 0 && (c & ~(4 * kLanes - 1)) < nvec)
+    sfrow[512 * (c / (4 * kLanes)) + ((c / kLanes) & 3)] = static_cast<uint8_t>(byte);
 }
 
 // ---------------------------------------------------------------- direct row kernels
@@ -191,7 +196,7 @@ __device__ __forceinline__ void group_quant_fp4(const RowGroup& grp, const Fp4Ou
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const int c = grp.t + grp.T * i;
-    if (c - (grp.t & 31) < nvec) store_vec_fp4<MX>(o, qrow, sfrow, c, nvec, v[i], inverse);   // warp-uniform
+    if (c - (grp.t & 31) < nvec) store_vec_fp4<MX>(qrow, sfrow, c, nvec, v[i], inverse);   // warp-uniform
   }
 }
 

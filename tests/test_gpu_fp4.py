@@ -44,7 +44,7 @@ def check_operand(got, x, kind):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("s,d", [(1, 8), (1, 16), (3, 24), (5, 40), (129, 128), (33, 264), (64, 1288), (300, 2048),
-                                 (2, 8192), (7, 8200), (5, 12288), (3, 49152)])
+                                 (2, 8192), (7, 8200), (5, 12288), (3, 49152), (2100, 1024), (2500, 3072)])
 def test_quant_rows(kind, s, d):
     rng = np.random.default_rng(s * 100003 + d)
     x = rand_bf16(rng, s, d)
@@ -105,7 +105,9 @@ def test_dequant_types(kind, dtype):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("s,d,form", [(1, 64, "batch"), (10, 264, "index"), (64, 1024, "batch"), (35, 2048, "w"),
-                                      (20, 1288, "w"), (6, 8192, "index"), (4, 9216, "batch"), (3, 20488, "w")])
+                                      (20, 1288, "w"), (6, 8192, "index"), (4, 9216, "batch"), (3, 20488, "w"),
+                                      (2500, 1024, "index"), (2200, 3072, "batch"), (2051, 2048, "w"),
+                                      (2300, 4096, "index")])
 def test_rms_mod_quant_equals_quant_of_h(kind, s, d, form):
     rng = np.random.default_rng(d + s)
     x = rand_bf16(rng, s, d, 0.5).to(DEV)

@@ -299,6 +299,103 @@ __global__ void __launch_bounds__(512) rows_fp4_kernel(const RmsArgs a, const Fp
   }
 }
 
+// ---------------------------------------------------------------- register-resident warp rows
+// The norm of many rows of 256 NV elements: one row per warp on the warp ring of rows.cuh (lane l holds
+// vectors 32 k + l), so that the per-row work (sums, reciprocal square root, scale) is shared by NV
+// vectors a lane instead of three, and no warp waits for another; the modulation of the CTA's middle row
+// and the norm weight are cached in shared memory (fill_mod_cache).  The sum of squares is the same
+// canonical tree.  Bound by instruction issue and latency: 16 warps (128 registers) measured 63 us at 32768 x 3072
+// mxfp4, 20 took 72 and 24 82 (spills), with one slot each
+// (it refills as soon as the row is in registers).
+
+// bf16(h) of one vector, and max |h| (float32, NaN above all) folded into amax.
+template <bool HAS_W>
+__device__ __forceinline__ uint4 rms_h_fp4(const uint4& xu, float2 inv2, const uint4& wu, const float2 (&s)[4],
+                                           const uint4& bu, float& amax) {
+  const uint32_t xw[4] = {xu.x, xu.y, xu.z, xu.w};
+  const uint32_t ww[4] = {wu.x, wu.y, wu.z, wu.w};
+  const uint32_t bw[4] = {bu.x, bu.y, bu.z, bu.w};
+  uint32_t hw[4];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    float2 t = mul2_rn(bf2_to_f2(xw[p]), inv2);
+    if constexpr (HAS_W) t = mul2_rn(t, bf2_to_f2(ww[p]));
+    const float2 h = add_f32_bf16x2(mul2_rn(t, s[p]), bw[p]);
+    amax = max3_abs_nan(amax, h.x, h.y);
+    hw[p] = f2_to_bf2(h);
+  }
+  return make_uint4(hw[0], hw[1], hw[2], hw[3]);
+}
+
+// The same with the modulation read from global memory, out of line: a row whose modulation row is not the
+// CTA's cached one.
+template <bool HAS_W>
+__device__ __noinline__ uint4 rms_h_fp4_global(const __nv_bfloat16* srow, const __nv_bfloat16* brow, int multiplier, int c,
+                                               uint4 xu, float inv, uint4 wu, float* amax) {
+  uint4 su = ld_v4(srow + 8 * c);
+  if (!multiplier)
+    su = make_uint4(one_plus_bf16x2(su.x), one_plus_bf16x2(su.y), one_plus_bf16x2(su.z), one_plus_bf16x2(su.w));
+  float2 s[4];
+  unpack_pairs(su, s);
+  float m = *amax;
+  const uint4 hu = rms_h_fp4<HAS_W>(xu, make_float2(inv, inv), wu, s, ld_v4(brow + 8 * c), m);
+  *amax = m;
+  return hu;
+}
+
+constexpr int kFp4NormWarps = 16;
+
+template <bool MX, int NV, bool HAS_W>
+__global__ void __launch_bounds__(32 * kFp4NormWarps, 1)
+    rms_mod_fp4_reg_kernel(const RmsArgs a, const WarpRingGeom g, const Fp4Out o) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int lane = threadIdx.x & 31;
+  float4* cache = mod_cache_of<NV>(smem, g);
+  const int64_t cm = fill_mod_cache<NV, HAS_W>(a, g, cache);
+  __syncthreads();
+  int64_t cur_m = -1, seg_end = -1;
+  auto src = [&](int64_t r) -> const void* { return a.x + r * a.ld_x; };
+  warp_row_loop_reg(
+      smem, g, a.S, src, [&](const uint8_t* slot, int64_t) { return load_row_regs<NV>(slot, lane); },
+      [&](int64_t row, RowRegs<NV>& r) {
+        const int64_t m = mod_row_of(a, row, cur_m, seg_end);
+        const float inv = row_inv_reg<NV>(r, a.eps);
+        float amax = 0.f;
+        if (m == cm) {
+          const float2 inv2 = make_float2(inv, inv);
+#pragma unroll
+          for (int k = 0; k < NV; ++k) {
+            const int c = 32 * k + lane;
+            float2 s[4];
+            uint4 bu, wu = make_uint4(0, 0, 0, 0);
+            mod_of<NV>(a, cache, true, m, c, s, bu);
+            if constexpr (HAS_W) wu = weight_of<NV>(cache, c);
+            r.v[k] = rms_h_fp4<HAS_W>(r.v[k], inv2, wu, s, bu, amax);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < NV; ++k) {
+            const int c = 32 * k + lane;
+            uint4 wu = make_uint4(0, 0, 0, 0);
+            if constexpr (HAS_W) wu = weight_of<NV>(cache, c);
+            r.v[k] = rms_h_fp4_global<HAS_W>(a.scale + m * a.ld_mod, a.shift + m * a.ld_mod, a.scale_is_multiplier, c,
+                                             r.v[k], inv, wu, &amax);
+          }
+        }
+        float inverse = 0.f;
+        if constexpr (!MX) {
+          // max |bf16(h)| = bf16(max |h|): rounding is monotone and symmetric (a NaN stays one)
+          const float top = __uint_as_float(warp_max_u32(__float_as_uint(amax)));
+          const float scale = row_scale_fp4(__bfloat16_as_ushort(__float2bfloat16_rn(top)), &inverse);
+          if (lane == 0) o.q_scale[row] = scale;
+        }
+        uint8_t* qrow = o.q + row * o.ld_q;
+        uint8_t* sfrow = o.sf + scale_row(row, o.words);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) store_vec_fp4<MX>(qrow, sfrow, 32 * k + lane, 32 * NV, r.v[k], inverse);
+      });
+}
+
 // ---------------------------------------------------------------- SwiGLU
 // act = bf16((gate * sigmoid(gate)) * up) as swiglu_kernel computes it, on its ring (the sigmoid table
 // is worth loading only once per CTA), quantised from registers.

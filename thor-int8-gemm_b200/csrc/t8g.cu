@@ -627,6 +627,7 @@ struct WarpLaunch {
   bool contiguous = false;
   bool padded = false;   // rows in 256-byte pieces at the padded pitch (reference-order reduction)
   size_t smem_budget = 216 * 1024;   // rings + tail
+  int stages = kWarpStages;          // slots per warp
 };
 
 template <typename K, typename A, typename... Extra>
@@ -639,7 +640,7 @@ int launch_warp_rows(K kern, const A& args, uint32_t row_bytes, int64_t rows, in
   g.row_bytes = row_bytes;
   g.padded = opt.padded ? 1 : 0;
   g.slot_bytes = ((opt.padded ? padded_row_bytes(row_bytes) : row_bytes) + 127u) & ~127u;
-  g.stages = kWarpStages;
+  g.stages = opt.stages;
   const int64_t budget = static_cast<int64_t>(opt.smem_budget - kWarpRingHeader) - static_cast<int64_t>(opt.tail_bytes);
   int64_t warps = budget / (static_cast<int64_t>(g.stages) * g.slot_bytes);
   if (warps > opt.max_warps) warps = opt.max_warps;

@@ -56,6 +56,9 @@ t8g::rows::Fp4Out fp4_out(void* q, int64_t ld_q, void* sf, float* q_scale, int64
     __VA_ARGS__;                                       \
   }
 
+// Rows from which the register-resident warp kernels run (rows of 256 NV elements).
+constexpr int64_t kFp4RegRows = 2048;
+
 // Launch a direct row kernel: T threads a row, as many rows a CTA as make 256 threads, and no more CTAs
 // than the device holds at a time (each group then takes several consecutive rows).
 template <typename K>
@@ -74,12 +77,33 @@ int launch_rows_fp4(K kern, const t8g::rows::RmsArgs& a, const t8g::rows::Fp4Out
 }
 
 template <int SRC>
-int dispatch_rows_fp4(const t8g::rows::RmsArgs& a, const t8g::rows::Fp4Out& o, int quant_kind, int sms, cudaStream_t st,
-                      const char* what) {
+int dispatch_rows_fp4(const t8g::rows::RmsArgs& a, const t8g::rows::Fp4Out& o, int quant_kind, int dev, int sms,
+                      cudaStream_t st, const char* what) {
   using namespace t8g::rows;
+  const bool mx = quant_kind == T8G_QUANT_MXFP4;
+  if constexpr (SRC != kFp4Plain) {
+    const int nv = reg_nv(a.D);
+    if (nv && a.S >= kFp4RegRows) {
+      constexpr bool W = SRC == kFp4NormWeight;
+      WarpLaunch l;
+      l.max_warps = kFp4NormWarps;
+      l.stages = 1;
+      l.contiguous = true;
+      l.tail_bytes = static_cast<size_t>((W ? 8 : 6) * a.D);   // fp32 multiplier + bf16 shift (+ bf16 weight)
+      l.smem_budget = kRowSmemLimit;
+      const uint32_t row_bytes = static_cast<uint32_t>(2 * a.D);
+      int rc = T8G_OK;
+      if (mx) {
+        T8G_DISPATCH_NV(nv, rc = launch_warp_rows(rms_mod_fp4_reg_kernel<true, NV, W>, a, row_bytes, a.S, dev, sms, st, l, what, o));
+      } else {
+        T8G_DISPATCH_NV(nv, rc = launch_warp_rows(rms_mod_fp4_reg_kernel<false, NV, W>, a, row_bytes, a.S, dev, sms, st, l, what, o));
+      }
+      return rc;
+    }
+  }
   const int T = row_shape(a.D).T;
   const int v = (a.D / 8 + T - 1) / T;
-  if (quant_kind == T8G_QUANT_MXFP4) {
+  if (mx) {
     T8G_DISPATCH_FP4_V(v, return launch_rows_fp4(rows_fp4_kernel<true, V, SRC>, a, o, T, sms, st, what))
   } else {
     T8G_DISPATCH_FP4_V(v, return launch_rows_fp4(rows_fp4_kernel<false, V, SRC>, a, o, T, sms, st, what))
@@ -276,7 +300,7 @@ int t8g_quant_rows_fp4(const void* x, int64_t ld_x, void* q, int64_t ld_q, void*
   a.ld_x = ld_x;
   a.S = S;
   a.D = static_cast<int>(D);
-  return dispatch_rows_fp4<kFp4Plain>(a, fp4_out(q, ld_q, sf, q_scale, S, D, quant_kind), quant_kind, info.sms, st,
+  return dispatch_rows_fp4<kFp4Plain>(a, fp4_out(q, ld_q, sf, q_scale, S, D, quant_kind), quant_kind, dev, info.sms, st,
                                       "quant_rows_fp4");
 }
 
@@ -312,8 +336,8 @@ int t8g_rms_mod_quant_fp4(const void* x, int64_t ld_x, const void* w, const void
   a.S = S;
   a.D = static_cast<int>(D);
   const Fp4Out o = fp4_out(q, ld_q, sf, q_scale, S, D, quant_kind);
-  return w ? dispatch_rows_fp4<kFp4NormWeight>(a, o, quant_kind, info.sms, st, "rms_mod_quant_fp4")
-           : dispatch_rows_fp4<kFp4Norm>(a, o, quant_kind, info.sms, st, "rms_mod_quant_fp4");
+  return w ? dispatch_rows_fp4<kFp4NormWeight>(a, o, quant_kind, dev, info.sms, st, "rms_mod_quant_fp4")
+           : dispatch_rows_fp4<kFp4Norm>(a, o, quant_kind, dev, info.sms, st, "rms_mod_quant_fp4");
 }
 
 int t8g_swiglu_quant_fp4(const void* gate, const void* up, int64_t ld_in, void* q, int64_t ld_q, void* sf, float* q_scale,

@@ -61,14 +61,22 @@ constexpr int64_t kFp4RegRows = 2048;
 
 // Launch a direct row kernel: T threads a row, as many rows a CTA as make 256 threads, and no more CTAs
 // than the device holds at a time (each group then takes several consecutive rows).
-template <typename K>
-int launch_rows_fp4(K kern, const t8g::rows::RmsArgs& a, const t8g::rows::Fp4Out& o, int T, int sms, cudaStream_t st,
+template <bool MX, int V, int SRC>
+int launch_rows_fp4(const t8g::rows::RmsArgs& a, const t8g::rows::Fp4Out& o, int T, int dev, int sms, cudaStream_t st,
                     const char* what) {
+  auto kern = t8g::rows::rows_fp4_kernel<MX, V, SRC>;
   const int groups = T <= 128 ? 256 / T : 1;
   const int threads = groups * T;
-  int occ = 0;
-  T8G_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, threads, 0), "occupancy query");
-  const int64_t held = static_cast<int64_t>(occ < 1 ? 1 : occ) * sms * groups;   // rows in work at a time
+  // resident CTAs per SM, looked up once per device and block size (a multiple of 32)
+  static std::atomic<int> occ_of[kMaxDevices][17] = {};
+  std::atomic<int>& known = occ_of[dev][threads / 32];
+  int occ = known.load(std::memory_order_relaxed);
+  if (occ == 0) {
+    T8G_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, threads, 0), "occupancy query");
+    occ = occ < 1 ? 1 : occ;
+    known.store(occ, std::memory_order_relaxed);
+  }
+  const int64_t held = static_cast<int64_t>(occ) * sms * groups;   // rows in work at a time
   const int64_t per_group = (a.S + held - 1) / held;
   const int64_t grid = (a.S + per_group * groups - 1) / (per_group * groups);
   kern<<<static_cast<unsigned>(grid), threads, 0, st>>>(a, o, T, per_group);
@@ -104,9 +112,9 @@ int dispatch_rows_fp4(const t8g::rows::RmsArgs& a, const t8g::rows::Fp4Out& o, i
   const int T = row_shape(a.D).T;
   const int v = (a.D / 8 + T - 1) / T;
   if (mx) {
-    T8G_DISPATCH_FP4_V(v, return launch_rows_fp4(rows_fp4_kernel<true, V, SRC>, a, o, T, sms, st, what))
+    T8G_DISPATCH_FP4_V(v, return (launch_rows_fp4<true, V, SRC>(a, o, T, dev, sms, st, what)))
   } else {
-    T8G_DISPATCH_FP4_V(v, return launch_rows_fp4(rows_fp4_kernel<false, V, SRC>, a, o, T, sms, st, what))
+    T8G_DISPATCH_FP4_V(v, return (launch_rows_fp4<false, V, SRC>(a, o, T, dev, sms, st, what)))
   }
 }
 

@@ -527,6 +527,14 @@ def _one_device(**tensors) -> None:
 
 
 def _fp4_operand(name: str, q: torch.Tensor, sf: torch.Tensor, kind: str):
+    try:
+        if q.dtype is torch.uint8 and sf.dtype is torch.uint8 and q.is_cuda and sf.is_cuda and sf.dim() == 1:
+            rows, half = q.shape
+            if ((q.stride(1) == 1 or not rows or not half) and sf.is_contiguous()
+                    and sf.shape[0] >= _fp4_scale_bytes(rows, 2 * half, kind)):
+                return rows, 2 * half
+    except (AttributeError, ValueError):
+        pass
     _need_cuda(name, q, torch.uint8, 2)
     rows, D = q.shape[0], 2 * q.shape[1]
     _need_cuda(f"{name}_sf", sf, torch.uint8, 1)
@@ -536,9 +544,19 @@ def _fp4_operand(name: str, q: torch.Tensor, sf: torch.Tensor, kind: str):
     return rows, D
 
 
-def _fp4_row_len(name: str, D: int) -> None:
-    if D % 8:
-        raise ValueError(f"{name} has rows of {D} elements, not a multiple of 8")
+def _fp4_bf16_rows(name: str, t: torch.Tensor):
+    """A CUDA bf16 matrix with rows of a multiple of 8 elements -> its shape."""
+    try:
+        if t.dtype is torch.bfloat16 and t.is_cuda:
+            S, D = t.shape
+            if not D % 8 and (t.stride(1) == 1 or not S or not D):
+                return S, D
+    except (AttributeError, ValueError):
+        pass
+    _need_cuda(name, t, torch.bfloat16, 2)
+    if t.shape[1] % 8:
+        raise ValueError(f"{name} has rows of {t.shape[1]} elements, not a multiple of 8")
+    return t.shape
 
 
 def quant_rows_fp4(x: torch.Tensor, kind: str = "nvfp4", stream=None):
@@ -548,9 +566,7 @@ def quant_rows_fp4(x: torch.Tensor, kind: str = "nvfp4", stream=None):
     e4m3 scale, and a power of two per row.  A block (mxfp4) or row (nvfp4) that holds a NaN or an
     infinity stands for NaN."""
     code = _fp4_code(kind)
-    _need_cuda("x", x, torch.bfloat16, 2)
-    S, D = x.shape
-    _fp4_row_len("x", D)
+    S, D = _fp4_bf16_rows("x", x)
     q, sf, q_scale = _fp4_empty(S, D, kind, x.device)
     idx = x.get_device()
     with _on(idx):
@@ -566,19 +582,23 @@ def dequant_rows_fp4(q: torch.Tensor, sf: torch.Tensor, q_scale: torch.Tensor | 
     """What a 4-bit matrix stands for: (code * block scale) * q_scale as bf16, fp16 or fp32 [S, D]."""
     code = _fp4_code(kind)
     S, D = _fp4_operand("q", q, sf, kind)
-    _fp4_row_len("q", D)
-    if q_scale is not None:
+    if D % 8:
+        raise ValueError(f"q has rows of {D} elements, not a multiple of 8")
+    idx = q.get_device()
+    if q_scale is not None and not _vector_ok(q_scale, torch.float32, (S,), idx):
         _need_cuda("q_scale", q_scale, torch.float32, 1)
         if q_scale.numel() != S or not q_scale.is_contiguous():
             raise ValueError("q_scale must be a contiguous float32 tensor with S elements")
     if out_dtype not in OUT_CODE:
         raise TypeError(f"out_dtype {out_dtype} is not one of {tuple(OUT_CODE)}")
-    _one_device(q=q, sf=sf, q_scale=q_scale)
+    if sf.get_device() != idx or (q_scale is not None and q_scale.get_device() != idx):
+        _one_device(q=q, sf=sf, q_scale=q_scale)
     out = torch.empty(S, D, dtype=out_dtype, device=q.device)
-    with _on(q.device):
-        rc = _lib.load().t8g_dequant_rows_fp4(_ptr(q), _pitch(q, 16), _ptr(sf), _ptr(q_scale), _ptr(out),
-                                              OUT_CODE[out_dtype], D, S, D, code, _stream_handle(q.device, stream))
-    _lib.check(rc)
+    with _on(idx):
+        rc = _lib.load().t8g_dequant_rows_fp4(q.data_ptr(), _pitch(q, 16), sf.data_ptr(), _ptr(q_scale), out.data_ptr(),
+                                              OUT_CODE[out_dtype], D, S, D, code, _stream_handle(idx, stream))
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -588,55 +608,65 @@ def rms_mod_quant_fp4(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor,
     """rms_mod_quant with 4-bit output -> (q, sf, q_scale): quant_rows_fp4 of its bf16 h, bit for
     bit, without storing h.  Values of mod_index are trusted to be rows of shift / scale."""
     code = _fp4_code(kind)
-    _need_cuda("x", x, torch.bfloat16, 2)
-    S, D = x.shape
-    _fp4_row_len("x", D)
-    shift2, scale2, rpm = _mod_args(x, shift, scale, mod_index, rows_per_mod)
-    if shift2.shape[0] != scale2.shape[0]:
-        raise ValueError(f"shift has {shift2.shape[0]} rows, scale {scale2.shape[0]}")
-    if mod_index is None and (rpm < 1 or (S and (S - 1) // rpm >= shift2.shape[0])):
-        raise ValueError(f"rows_per_mod={rpm} maps rows past the {shift2.shape[0]} modulation rows")
+    S, D = _fp4_bf16_rows("x", x)
+    idx = x.get_device()
+    if not (rows_per_mod and mod_index is None and shift.dim() == 2 and scale.dim() == 2 and shift.shape == scale.shape
+            and shift.shape[1] == D and shift.dtype is torch.bfloat16 and scale.dtype is torch.bfloat16
+            and shift.stride() == scale.stride() and (not D or shift.stride(1) == 1) and shift.get_device() == idx
+            and scale.get_device() == idx):
+        shift, scale, rows_per_mod = _mod_args(x, shift, scale, mod_index, rows_per_mod)
+        if shift.shape[0] != scale.shape[0]:
+            raise ValueError(f"shift has {shift.shape[0]} rows, scale {scale.shape[0]}")
+        _one_device(x=x, shift=shift, scale=scale, mod_index=mod_index)
+    rpm = int(rows_per_mod)
+    if mod_index is None and (rpm < 1 or (S and (S - 1) // rpm >= shift.shape[0])):
+        raise ValueError(f"rows_per_mod={rpm} maps rows past the {shift.shape[0]} modulation rows")
     if w is not None:
         _need_cuda("w", w, torch.bfloat16, 1)
         if w.numel() != D:
             raise ValueError("w must have D elements")
-    _one_device(x=x, shift=shift, scale=scale, w=w, mod_index=mod_index)
+        _one_device(x=x, w=w)
     q, sf, q_scale = _fp4_empty(S, D, kind, x.device)
-    with _on(x.device):
+    with _on(idx):
         rc = _lib.load().t8g_rms_mod_quant_fp4(
-            _ptr(x), _pitch(x, 8), _ptr(w), _ptr(shift2), _ptr(scale2), _pitch(shift2, 8), _ptr(mod_index), rpm,
-            int(scale_is_multiplier), float(eps), _ptr(q), _pitch(q, 16), _ptr(sf), _ptr(q_scale), S, D, code,
-            _stream_handle(x.device, stream))
-    _lib.check(rc)
+            x.data_ptr(), _pitch(x, 8), _ptr(w), shift.data_ptr(), scale.data_ptr(), _pitch(shift, 8), _ptr(mod_index), rpm,
+            int(scale_is_multiplier), float(eps), q.data_ptr(), _pitch(q, 16), sf.data_ptr(), _ptr(q_scale), S, D, code,
+            _stream_handle(idx, stream))
+    if rc:
+        _lib.check(rc)
     return q, sf, q_scale
 
 
 def swiglu_quant_fp4(gate: torch.Tensor, up: torch.Tensor, kind: str = "nvfp4", stream=None):
     """swiglu_quant with 4-bit output -> (q, sf, q_scale): quant_rows_fp4 of act = bf16(silu(gate) *
     up), bit for bit, without storing act."""
-    code = _fp4_code(kind)
-    _need_cuda("gate", gate, torch.bfloat16, 2)
+    M, F = _fp4_bf16_rows("gate", gate)
     _need_cuda("up", up, torch.bfloat16, 2)
-    M, F = gate.shape
     if gate.shape != up.shape or (M > 1 and gate.stride(0) != up.stride(0)):
         raise ValueError("gate and up must have the same shape and strides")
-    _fp4_row_len("gate", F)
     _one_device(gate=gate, up=up)
-    q, sf, q_scale = _fp4_empty(M, F, kind, gate.device)
-    with _on(gate.device):
-        rc = _lib.load().t8g_swiglu_quant_fp4(_ptr(gate), _ptr(up), _pitch(gate, 8), _ptr(q), _pitch(q, 16), _ptr(sf),
-                                              _ptr(q_scale), M, F, code, _stream_handle(gate.device, stream))
-    _lib.check(rc)
+    return _swiglu_fp4(gate.data_ptr(), up.data_ptr(), _pitch(gate, 8), M, F, kind, gate.device, stream)
+
+
+def _swiglu_fp4(gate: int, up: int, ld: int, M: int, F: int, kind: str, device, stream):
+    code = _fp4_code(kind)
+    q, sf, q_scale = _fp4_empty(M, F, kind, device)
+    idx = device.index
+    with _on(idx):
+        rc = _lib.load().t8g_swiglu_quant_fp4(gate, up, ld, q.data_ptr(), _pitch(q, 16), sf.data_ptr(), _ptr(q_scale), M, F,
+                                              code, _stream_handle(idx, stream))
+    if rc:
+        _lib.check(rc)
     return q, sf, q_scale
 
 
 def swiglu_quant_fp4_fc1(y: torch.Tensor, kind: str = "nvfp4", stream=None):
-    """swiglu_quant_fp4 of a [M, 2F] fc1 output whose first half is the gate."""
-    _need_cuda("y", y, torch.bfloat16, 2)
-    if y.shape[1] % 2:
-        raise ValueError(f"y must be [M, 2F], got {tuple(y.shape)}")
-    F = y.shape[-1] // 2
-    return swiglu_quant_fp4(y[:, :F], y[:, F:], kind=kind, stream=stream)
+    """swiglu_quant_fp4 of a [M, 2F] fc1 output whose first half is the gate (read in place)."""
+    M, F2 = _fp4_bf16_rows("y", y)
+    if F2 % 16:
+        raise ValueError(f"y has rows of {F2} elements: two halves of a multiple of 8 are wanted")
+    p = y.data_ptr()
+    return _swiglu_fp4(p, p + F2 if p else p, _pitch(y, 8), M, F2 // 2, kind, y.device, stream)   # F2 / 2 bf16 elements
 
 
 def _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype):
@@ -741,14 +771,17 @@ def gemm_fp4_gated(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: t
     rows of gate) or m // rows_per_gate; out may be res itself (in-place update)."""
     code = _fp4_code(kind)
     M, N, K, nws, nb = _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, torch.bfloat16)
-    _need_cuda("res", res, torch.bfloat16, 2)
-    if tuple(res.shape) != (M, N):
-        raise ValueError(f"res has shape {tuple(res.shape)}, expected {(M, N)}")
     if gate.dim() == 1:
         gate = gate.view(1, -1)
-    _need_cuda("gate", gate, torch.bfloat16, 2)
-    if gate.shape[1] != N or gate.shape[0] < 1:
-        raise ValueError(f"gate must be [n_gate, {N}], got {tuple(gate.shape)}")
+    if not (res.dtype is torch.bfloat16 and gate.dtype is torch.bfloat16 and res.dim() == 2 and gate.dim() == 2
+            and res.shape[0] == M and res.shape[1] == N and gate.shape[1] == N and gate.shape[0] and res.is_cuda
+            and gate.is_cuda and (not M or not N or (res.stride(1) == 1 and gate.stride(1) == 1))):
+        _need_cuda("res", res, torch.bfloat16, 2)
+        if tuple(res.shape) != (M, N):
+            raise ValueError(f"res has shape {tuple(res.shape)}, expected {(M, N)}")
+        _need_cuda("gate", gate, torch.bfloat16, 2)
+        if gate.shape[1] != N or gate.shape[0] < 1:
+            raise ValueError(f"gate must be [n_gate, {N}], got {tuple(gate.shape)}")
     if gate_index is not None:
         _need_cuda("gate_index", gate_index, torch.int32, 1)
         if gate_index.numel() != M or not gate_index.is_contiguous():

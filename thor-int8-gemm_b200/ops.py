@@ -36,6 +36,26 @@ def _stream_handle(device, stream=None) -> int:
     return int(stream)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _call(fn, idx: int, *args) -> None:
+    """fn(*args, current stream or the given one) with CUDA device `idx` current; `args` ends with the
+    stream (None: torch's current stream of that device).  Raises on a nonzero status."""
+    stream = args[-1]
+    if stream is None and _raw_stream is not None:
+        handle = _raw_stream(idx)
+    else:
+        handle = _stream_handle(idx, stream)
+    if _current_device() == idx:
+        rc = fn(*args[:-1], handle)
+    else:
+        with _on(idx):
+            rc = fn(*args[:-1], handle)
+    if rc:
+        _lib.check(rc)
+
+
 class _on:
     """Makes `device` the current CUDA device inside the block (a no-op when it already is)."""
     __slots__ = ("idx", "prev")
@@ -515,9 +535,8 @@ def _fp4_empty(S: int, D: int, kind: str, device):
 
 def _pitch(t: torch.Tensor, multiple: int) -> int:
     """Row stride in elements; a single row has none of its own."""
-    if t.shape[0] > 1:
-        return t.stride(0)
-    return -(-t.shape[1] // multiple) * multiple
+    rows, width = t.shape
+    return t.stride(0) if rows > 1 else -(-width // multiple) * multiple
 
 
 def _one_device(**tensors) -> None:
@@ -569,11 +588,8 @@ def quant_rows_fp4(x: torch.Tensor, kind: str = "nvfp4", stream=None):
     S, D = _fp4_bf16_rows("x", x)
     q, sf, q_scale = _fp4_empty(S, D, kind, x.device)
     idx = x.get_device()
-    with _on(idx):
-        rc = _lib.load().t8g_quant_rows_fp4(x.data_ptr(), _pitch(x, 8), q.data_ptr(), _pitch(q, 16), sf.data_ptr(),
-                                            _ptr(q_scale), S, D, code, _stream_handle(idx, stream))
-    if rc:
-        _lib.check(rc)
+    _call(_lib.load().t8g_quant_rows_fp4, idx, x.data_ptr(), _pitch(x, 8), q.data_ptr(), _pitch(q, 16), sf.data_ptr(),
+          _ptr(q_scale), S, D, code, stream)
     return q, sf, q_scale
 
 
@@ -594,11 +610,8 @@ def dequant_rows_fp4(q: torch.Tensor, sf: torch.Tensor, q_scale: torch.Tensor | 
     if sf.get_device() != idx or (q_scale is not None and q_scale.get_device() != idx):
         _one_device(q=q, sf=sf, q_scale=q_scale)
     out = torch.empty(S, D, dtype=out_dtype, device=q.device)
-    with _on(idx):
-        rc = _lib.load().t8g_dequant_rows_fp4(q.data_ptr(), _pitch(q, 16), sf.data_ptr(), _ptr(q_scale), out.data_ptr(),
-                                              OUT_CODE[out_dtype], D, S, D, code, _stream_handle(idx, stream))
-    if rc:
-        _lib.check(rc)
+    _call(_lib.load().t8g_dequant_rows_fp4, idx, q.data_ptr(), _pitch(q, 16), sf.data_ptr(), _ptr(q_scale),
+          out.data_ptr(), OUT_CODE[out_dtype], D, S, D, code, stream)
     return out
 
 
@@ -627,13 +640,9 @@ def rms_mod_quant_fp4(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor,
             raise ValueError("w must have D elements")
         _one_device(x=x, w=w)
     q, sf, q_scale = _fp4_empty(S, D, kind, x.device)
-    with _on(idx):
-        rc = _lib.load().t8g_rms_mod_quant_fp4(
-            x.data_ptr(), _pitch(x, 8), _ptr(w), shift.data_ptr(), scale.data_ptr(), _pitch(shift, 8), _ptr(mod_index), rpm,
-            int(scale_is_multiplier), float(eps), q.data_ptr(), _pitch(q, 16), sf.data_ptr(), _ptr(q_scale), S, D, code,
-            _stream_handle(idx, stream))
-    if rc:
-        _lib.check(rc)
+    _call(_lib.load().t8g_rms_mod_quant_fp4, idx, x.data_ptr(), _pitch(x, 8), _ptr(w), shift.data_ptr(),
+          scale.data_ptr(), _pitch(shift, 8), _ptr(mod_index), rpm, int(scale_is_multiplier), float(eps), q.data_ptr(),
+          _pitch(q, 16), sf.data_ptr(), _ptr(q_scale), S, D, code, stream)
     return q, sf, q_scale
 
 
@@ -651,12 +660,8 @@ def swiglu_quant_fp4(gate: torch.Tensor, up: torch.Tensor, kind: str = "nvfp4", 
 def _swiglu_fp4(gate: int, up: int, ld: int, M: int, F: int, kind: str, device, stream):
     code = _fp4_code(kind)
     q, sf, q_scale = _fp4_empty(M, F, kind, device)
-    idx = device.index
-    with _on(idx):
-        rc = _lib.load().t8g_swiglu_quant_fp4(gate, up, ld, q.data_ptr(), _pitch(q, 16), sf.data_ptr(), _ptr(q_scale), M, F,
-                                              code, _stream_handle(idx, stream))
-    if rc:
-        _lib.check(rc)
+    _call(_lib.load().t8g_swiglu_quant_fp4, device.index, gate, up, ld, q.data_ptr(), _pitch(q, 16), sf.data_ptr(),
+          _ptr(q_scale), M, F, code, stream)
     return q, sf, q_scale
 
 
@@ -750,14 +755,9 @@ def gemm_fp4(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: torch.T
         if tuple(out.shape) != (M, N):
             raise ValueError(f"out has shape {tuple(out.shape)}, expected {(M, N)}")
         _one_device(x=x, out=out)
-    idx = x.get_device()
-    with _on(idx):
-        rc = _lib.load().t8g_gemm_fp4(
-            x.data_ptr(), x_sf.data_ptr(), _ptr(x_scale), w.data_ptr(), w_sf.data_ptr(), _ptr(w_scale), nws,
-            bias.data_ptr() if nb else None, nb, out.data_ptr(), OUT_CODE[out_dtype], M, N, K, _pitch(x, 16),
-            _pitch(w, 16), _pitch(out, 16 // out_dtype.itemsize), code, _stream_handle(idx, stream))
-    if rc:
-        _lib.check(rc)
+    _call(_lib.load().t8g_gemm_fp4, x.get_device(), x.data_ptr(), x_sf.data_ptr(), _ptr(x_scale), w.data_ptr(),
+          w_sf.data_ptr(), _ptr(w_scale), nws, bias.data_ptr() if nb else None, nb, out.data_ptr(), OUT_CODE[out_dtype],
+          M, N, K, _pitch(x, 16), _pitch(w, 16), _pitch(out, 16 // out_dtype.itemsize), code, stream)
     return out
 
 
@@ -805,14 +805,10 @@ def gemm_fp4_gated(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: t
     if (res.get_device() != idx or gate.get_device() != idx or out.get_device() != idx
             or (gate_index is not None and gate_index.get_device() != idx)):
         _one_device(x=x, res=res, gate=gate, gate_index=gate_index, out=out)
-    with _on(idx):
-        rc = _lib.load().t8g_gemm_fp4_gated(
-            x.data_ptr(), x_sf.data_ptr(), _ptr(x_scale), w.data_ptr(), w_sf.data_ptr(), _ptr(w_scale), nws,
-            bias.data_ptr() if nb else None, nb, res.data_ptr(), _pitch(res, 8), gate.data_ptr(), _pitch(gate, 8),
-            _ptr(gate_index), rpg, out.data_ptr(), M, N, K, _pitch(x, 16), _pitch(w, 16), _pitch(out, 8), code,
-            _stream_handle(idx, stream))
-    if rc:
-        _lib.check(rc)
+    _call(_lib.load().t8g_gemm_fp4_gated, idx, x.data_ptr(), x_sf.data_ptr(), _ptr(x_scale), w.data_ptr(),
+          w_sf.data_ptr(), _ptr(w_scale), nws, bias.data_ptr() if nb else None, nb, res.data_ptr(), _pitch(res, 8),
+          gate.data_ptr(), _pitch(gate, 8), _ptr(gate_index), rpg, out.data_ptr(), M, N, K, _pitch(x, 16), _pitch(w, 16),
+          _pitch(out, 8), code, stream)
     return out
 
 

@@ -152,7 +152,8 @@ def tolerance(xv, wv, k, ref, dtype):
 
 
 SHAPES = [(1, 64, 64), (1, 1, 8), (3, 7, 24), (128, 64, 256), (5, 130, 520), (64, 192, 1024), (130, 257, 2104),
-          (256, 512, 768), (333, 1000, 264), (1, 1024, 4096), (300, 300, 4104), (700, 2304, 640)]
+          (256, 512, 768), (333, 1000, 264), (300, 5, 520), (300, 9, 264),
+          (2100, 1003, 136), (1, 1024, 4096), (300, 300, 4104), (700, 2304, 640)]
 
 
 @pytest.mark.parametrize("kind", KINDS)

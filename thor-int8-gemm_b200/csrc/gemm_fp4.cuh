@@ -444,6 +444,21 @@ __device__ __forceinline__ GatedSlice gated_prefetch(const Args& args, uint8_t (
   return g;
 }
 
+// The columns of a staged piece row past its last whole 16 bytes before N: `left` columns from n on.
+template <int OUT>
+__device__ __noinline__ void store_tail(const Args& args, const uint8_t* buf, int lane, int row0, int n, int left) {
+  constexpr int kBytes = OutTraits<OUT>::kBytes;
+  constexpr int kPer = 16 / kBytes;
+  const uint8_t* last = buf + lane * 128 + ((left / kPer) ^ (lane & 7)) * 16;
+  uint8_t* out = static_cast<uint8_t*>(args.out) + (static_cast<int64_t>(row0 + lane) * args.ld_out + n + left / kPer * kPer) * kBytes;
+  for (int j = 0; j < left % kPer; ++j) {
+    if constexpr (kBytes == 4)
+      reinterpret_cast<uint32_t*>(out)[j] = reinterpret_cast<const uint32_t*>(last)[j];
+    else
+      reinterpret_cast<uint16_t*>(out)[j] = reinterpret_cast<const uint16_t*>(last)[j];
+  }
+}
+
 // Epilogue of a warp's 32 x 128 slice of a tile (columns n0 .. of the output, `half` of the tile).
 // `shared`: this half holds the columns that the other accumulator uses too, its last ones if half is
 // 1 and its first if it is 0; they are read first and `shared_bar` (the leader's, a cluster
@@ -552,6 +567,11 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
       __syncwarp();
 #pragma unroll
       for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) * 16)) = o[q];
+      // TMA stores whole 16-byte pieces: the map ends at the last whole one before N, and the columns
+      // after it are stored one by one (what lies past N is not this call's to write)
+      constexpr int kPer = 16 / OutTraits<OUT>::kBytes;
+      const int left = cols - c * kCols;
+      if (left < kCols && left % kPer != 0 && row0 + lane < args.M) store_tail<OUT>(args, buf, lane, row0, n0 + c * kCols, left);
     }
     fence_proxy_async_smem();
     __syncwarp();

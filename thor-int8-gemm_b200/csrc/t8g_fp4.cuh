@@ -195,8 +195,8 @@ int launch_gemm_fp4_pair(const Fp4Gemm& p, const t8g::gemm4::Args& args, int dev
   const CUtensorMapDataType out_dt = OUT == kOutF32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                      : OUT == kOutF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  // 32 rows of 128 bytes: 64 two-byte or 32 four-byte columns
-  if ((rc = encode_2d(&to, out_dt, args.out, p.N, p.M, args.ld_out * esz, 128 / esz, 32, CU_TENSOR_MAP_SWIZZLE_128B)))
+  // 32 rows of 128 bytes: 64 two-byte or 32 four-byte columns, up to N's last whole 16-byte piece
+  if ((rc = encode_2d(&to, out_dt, args.out, p.N / (16 / esz) * (16 / esz), p.M, args.ld_out * esz, 128 / esz, 32, CU_TENSOR_MAP_SWIZZLE_128B)))
     return rc;
   const int64_t tiles = ((p.M + 255) / 256) * ((p.N + 255) / 256);
   if (tiles >= (int64_t(1) << 31)) return fail(T8G_ERR_UNSUPPORTED, "gemm_fp4: too many tiles");
@@ -216,7 +216,8 @@ int launch_gemm_fp4_pair(const Fp4Gemm& p, const t8g::gemm4::Args& args, int dev
 //   the pair kernel has a floor of 7 to 10 us and then the full rate; it runs above 64 rows when its
 //   256 x 256 tiles occupy more than a quarter of the SMs (128 x 9216 x 3072: 10.2 us, 11.9 with the small
 //   kernel), and above 128 rows also when K is too short to be worth splitting (at most 8 stages:
-//   256 x 1024 x 1024 7.5 us against 8.3, but 256 x 3072 x 12288 20.5 against 18.3);
+//   256 x 1024 x 1024 7.5 us against 8.3, but 256 x 3072 x 12288 20.5 against 18.3); its stores want a whole
+//   16-byte piece of columns;
 //   the small kernel takes the tile width and the power-of-two split that bring the CTAs nearest to
 //   one an SM (1 x 9216 x 3072: 72 tiles x 2 7.3 us, x 1 8.5, x 4 10.5; 1 x 3072 x 3072: 24 x 4 5.8,
 //   x 8 6.6), 128 columns where both widths come equally near (1 x 9216 x 3072: 144 x 1 of 64 columns
@@ -235,7 +236,8 @@ SmallPlan small_plan(int64_t M, int64_t N, int tbn, int kstages, int sms) {
 template <bool MX, int OUT>
 int launch_gemm_fp4(const Fp4Gemm& p, const t8g::gemm4::Args& args, int dev, int sms, cudaStream_t st) {
   const bool many = (p.M + 255) / 256 * ((p.N + 255) / 256) * 8 > sms;
-  if ((p.M > 64 && many) || (p.M > 128 && args.kstages <= 8)) return launch_gemm_fp4_pair<MX, OUT>(p, args, dev, sms, st);
+  if (((p.M > 64 && many) || (p.M > 128 && args.kstages <= 8)) && p.N >= 8)   // a whole 16-byte piece to store
+    return launch_gemm_fp4_pair<MX, OUT>(p, args, dev, sms, st);
   const SmallPlan w = small_plan(p.M, p.N, 128, args.kstages, sms), n = small_plan(p.M, p.N, 64, args.kstages, sms);
   if (n.ctas > w.ctas || (n.ctas == w.ctas && p.M > 64))
     return launch_gemm_fp4_small<MX, OUT, 64>(p, args, n.split, dev, st);

@@ -16,6 +16,14 @@ dtypes), at run time the op calls the CUDA kernel on the current stream.
     t8g::swiglu_quant(y, kind) -> (q, q_scale)                     (y = [M, 2F] fc1 output)
     t8g::gemm_swiglu(x, w_il, x_scale, w_scale_il, bias_il?) -> act  (fc1 + SwiGLU epilogue)
     t8g::gemm_gated(x, w, x_scale, w_scale, bias?, res, gate, rows_per_gate) -> res + gate * y
+  and of the microscaled 4-bit formats (kind "mxfp4" / "nvfp4"; q_scale is empty for mxfp4):
+    t8g::quant_rows_fp4(x, kind) -> (q, sf, q_scale)
+    t8g::rms_mod_quant_fp4(x, shift, scale, w?, mod_index?, rows_per_mod, scale_is_multiplier, eps,
+                           kind) -> (q, sf, q_scale)
+    t8g::swiglu_quant_fp4(y, kind) -> (q, sf, q_scale)
+    t8g::gemm_fp4(x, w, x_sf, w_sf, x_scale?, w_scale?, bias?, kind, out_dtype) -> out
+    t8g::gemm_fp4_gated(x, w, x_sf, w_sf, x_scale?, w_scale?, bias?, res, gate, rows_per_gate, kind)
+                           -> res + gate * y
 """
 from __future__ import annotations
 
@@ -134,5 +142,91 @@ def gemm_gated(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor, w_scale:
 @gemm_gated.register_fake
 def _(x, w, x_scale, w_scale, bias, res, gate, rows_per_gate):
     torch._check(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1], lambda: "x [M, K], w [N, K]")
+    torch._check(res.shape[0] == x.shape[0] and res.shape[1] == w.shape[0], lambda: "res must be [M, N]")
+    return res.new_empty(res.shape, dtype=torch.bfloat16)
+
+
+# ---------------------------------------------------------------- microscaled 4-bit formats
+# A custom op returns tensors, so the absent row scale of mxfp4 is an empty one; the products take an
+# empty scale as none.
+def _fp4_result(q, sf, q_scale):
+    return q, sf, q_scale if q_scale is not None else q.new_empty((0,), dtype=torch.float32)
+
+
+def _fp4_fake(x, S, D, kind):
+    torch._check(D % 8 == 0, lambda: "rows must be a multiple of 8 elements")
+    pitch = (D + 31) // 32 * 16
+    q = x.new_empty_strided((S, D // 2), (pitch, 1), dtype=torch.uint8)
+    sf = x.new_empty((ops.fp4_scale_bytes(S, D, kind),), dtype=torch.uint8)
+    return q, sf, x.new_empty((S if kind == "nvfp4" else 0,), dtype=torch.float32)
+
+
+def _none_if_empty(t):
+    return None if t is None or t.numel() == 0 else t
+
+
+@torch.library.custom_op("t8g::quant_rows_fp4", mutates_args=())
+def quant_rows_fp4(x: torch.Tensor, kind: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _fp4_result(*ops.quant_rows_fp4(x, kind))
+
+
+@quant_rows_fp4.register_fake
+def _(x, kind):
+    torch._check(x.dim() == 2, lambda: "x must be 2-D")
+    return _fp4_fake(x, x.shape[0], x.shape[1], kind)
+
+
+@torch.library.custom_op("t8g::rms_mod_quant_fp4", mutates_args=())
+def rms_mod_quant_fp4(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor, w: Optional[torch.Tensor],
+                      mod_index: Optional[torch.Tensor], rows_per_mod: int, scale_is_multiplier: bool, eps: float,
+                      kind: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _fp4_result(*ops.rms_mod_quant_fp4(x, shift, scale, w=w, mod_index=mod_index,
+                                              rows_per_mod=rows_per_mod if mod_index is None else None,
+                                              scale_is_multiplier=scale_is_multiplier, eps=eps, kind=kind))
+
+
+@rms_mod_quant_fp4.register_fake
+def _(x, shift, scale, w, mod_index, rows_per_mod, scale_is_multiplier, eps, kind):
+    torch._check(x.dim() == 2, lambda: "x must be 2-D")
+    return _fp4_fake(x, x.shape[0], x.shape[1], kind)
+
+
+@torch.library.custom_op("t8g::swiglu_quant_fp4", mutates_args=())
+def swiglu_quant_fp4(y: torch.Tensor, kind: str) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _fp4_result(*ops.swiglu_quant_fp4_fc1(y, kind))
+
+
+@swiglu_quant_fp4.register_fake
+def _(y, kind):
+    torch._check(y.dim() == 2 and y.shape[1] % 2 == 0, lambda: "y must be [M, 2F]")
+    return _fp4_fake(y, y.shape[0], y.shape[1] // 2, kind)
+
+
+@torch.library.custom_op("t8g::gemm_fp4", mutates_args=())
+def gemm_fp4(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: torch.Tensor, x_scale: Optional[torch.Tensor],
+             w_scale: Optional[torch.Tensor], bias: Optional[torch.Tensor], kind: str,
+             out_dtype: torch.dtype) -> torch.Tensor:
+    return ops.gemm_fp4(x, w, x_sf, w_sf, _none_if_empty(x_scale), _none_if_empty(w_scale), bias, kind=kind,
+                        out_dtype=out_dtype)
+
+
+@gemm_fp4.register_fake
+def _(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype):
+    torch._check(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1], lambda: "x [M, K / 2], w [N, K / 2]")
+    per = 16 // out_dtype.itemsize
+    return x.new_empty_strided((x.shape[0], w.shape[0]), ((w.shape[0] + per - 1) // per * per, 1), dtype=out_dtype)
+
+
+@torch.library.custom_op("t8g::gemm_fp4_gated", mutates_args=())
+def gemm_fp4_gated(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: torch.Tensor,
+                   x_scale: Optional[torch.Tensor], w_scale: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+                   res: torch.Tensor, gate: torch.Tensor, rows_per_gate: int, kind: str) -> torch.Tensor:
+    return ops.gemm_fp4_gated(x, w, x_sf, w_sf, _none_if_empty(x_scale), _none_if_empty(w_scale), bias, res, gate,
+                              rows_per_gate=rows_per_gate, kind=kind)
+
+
+@gemm_fp4_gated.register_fake
+def _(x, w, x_sf, w_sf, x_scale, w_scale, bias, res, gate, rows_per_gate, kind):
+    torch._check(x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1], lambda: "x [M, K / 2], w [N, K / 2]")
     torch._check(res.shape[0] == x.shape[0] and res.shape[1] == w.shape[0], lambda: "res must be [M, N]")
     return res.new_empty(res.shape, dtype=torch.bfloat16)

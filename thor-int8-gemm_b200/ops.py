@@ -533,9 +533,8 @@ def _fp4_empty(S: int, D: int, kind: str, device):
     return q, sf, q_scale
 
 
-def _pitch(t: torch.Tensor, multiple: int) -> int:
-    """Row stride in elements; a single row has none of its own."""
-    rows, width = t.shape
+def _pitch(t: torch.Tensor, rows: int, width: int, multiple: int) -> int:
+    """Row stride in elements of a [rows, width] matrix; a single row has none of its own."""
     return t.stride(0) if rows > 1 else -(-width // multiple) * multiple
 
 
@@ -588,8 +587,8 @@ def quant_rows_fp4(x: torch.Tensor, kind: str = "nvfp4", stream=None):
     S, D = _fp4_bf16_rows("x", x)
     q, sf, q_scale = _fp4_empty(S, D, kind, x.device)
     idx = x.get_device()
-    _call(_lib.load().t8g_quant_rows_fp4, idx, x.data_ptr(), _pitch(x, 8), q.data_ptr(), _pitch(q, 16), sf.data_ptr(),
-          _ptr(q_scale), S, D, code, stream)
+    _call(_lib.load().t8g_quant_rows_fp4, idx, x.data_ptr(), _pitch(x, S, D, 8), q.data_ptr(), _pitch(q, S, D // 2, 16),
+          sf.data_ptr(), _ptr(q_scale), S, D, code, stream)
     return q, sf, q_scale
 
 
@@ -610,7 +609,7 @@ def dequant_rows_fp4(q: torch.Tensor, sf: torch.Tensor, q_scale: torch.Tensor | 
     if sf.get_device() != idx or (q_scale is not None and q_scale.get_device() != idx):
         _one_device(q=q, sf=sf, q_scale=q_scale)
     out = torch.empty(S, D, dtype=out_dtype, device=q.device)
-    _call(_lib.load().t8g_dequant_rows_fp4, idx, q.data_ptr(), _pitch(q, 16), sf.data_ptr(), _ptr(q_scale),
+    _call(_lib.load().t8g_dequant_rows_fp4, idx, q.data_ptr(), _pitch(q, S, D // 2, 16), sf.data_ptr(), _ptr(q_scale),
           out.data_ptr(), OUT_CODE[out_dtype], D, S, D, code, stream)
     return out
 
@@ -640,9 +639,9 @@ def rms_mod_quant_fp4(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor,
             raise ValueError("w must have D elements")
         _one_device(x=x, w=w)
     q, sf, q_scale = _fp4_empty(S, D, kind, x.device)
-    _call(_lib.load().t8g_rms_mod_quant_fp4, idx, x.data_ptr(), _pitch(x, 8), _ptr(w), shift.data_ptr(),
-          scale.data_ptr(), _pitch(shift, 8), _ptr(mod_index), rpm, int(scale_is_multiplier), float(eps), q.data_ptr(),
-          _pitch(q, 16), sf.data_ptr(), _ptr(q_scale), S, D, code, stream)
+    _call(_lib.load().t8g_rms_mod_quant_fp4, idx, x.data_ptr(), _pitch(x, S, D, 8), _ptr(w), shift.data_ptr(),
+          scale.data_ptr(), _pitch(shift, shift.shape[0], D, 8), _ptr(mod_index), rpm, int(scale_is_multiplier), float(eps),
+          q.data_ptr(), _pitch(q, S, D // 2, 16), sf.data_ptr(), _ptr(q_scale), S, D, code, stream)
     return q, sf, q_scale
 
 
@@ -654,13 +653,13 @@ def swiglu_quant_fp4(gate: torch.Tensor, up: torch.Tensor, kind: str = "nvfp4", 
     if gate.shape != up.shape or (M > 1 and gate.stride(0) != up.stride(0)):
         raise ValueError("gate and up must have the same shape and strides")
     _one_device(gate=gate, up=up)
-    return _swiglu_fp4(gate.data_ptr(), up.data_ptr(), _pitch(gate, 8), M, F, kind, gate.device, stream)
+    return _swiglu_fp4(gate.data_ptr(), up.data_ptr(), _pitch(gate, M, F, 8), M, F, kind, gate.device, stream)
 
 
 def _swiglu_fp4(gate: int, up: int, ld: int, M: int, F: int, kind: str, device, stream):
     code = _fp4_code(kind)
     q, sf, q_scale = _fp4_empty(M, F, kind, device)
-    _call(_lib.load().t8g_swiglu_quant_fp4, device.index, gate, up, ld, q.data_ptr(), _pitch(q, 16), sf.data_ptr(),
+    _call(_lib.load().t8g_swiglu_quant_fp4, device.index, gate, up, ld, q.data_ptr(), _pitch(q, M, F // 2, 16), sf.data_ptr(),
           _ptr(q_scale), M, F, code, stream)
     return q, sf, q_scale
 
@@ -671,26 +670,34 @@ def swiglu_quant_fp4_fc1(y: torch.Tensor, kind: str = "nvfp4", stream=None):
     if F2 % 16:
         raise ValueError(f"y has rows of {F2} elements: two halves of a multiple of 8 are wanted")
     p = y.data_ptr()
-    return _swiglu_fp4(p, p + F2 if p else p, _pitch(y, 8), M, F2 // 2, kind, y.device, stream)   # F2 / 2 bf16 elements
+    # the up half starts F2 / 2 elements of two bytes in
+    return _swiglu_fp4(p, p + F2 if p else p, _pitch(y, M, F2, 8), M, F2 // 2, kind, y.device, stream)
 
 
 def _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype):
-    """Argument rules of the 4-bit products -> (M, N, K, w_scale numel, bias numel).  The common case
-    is checked cheaply, all tensors on one device; anything else goes to _fp4_product_explain,
-    which raises the precise error or accepts the call."""
+    """Argument rules of the 4-bit products -> (device, M, N, K, w_scale numel, bias numel).  The common
+    case is checked cheaply; anything else goes to _fp4_product_explain, which raises the precise
+    error or accepts the call."""
+    u8, f32 = torch.uint8, torch.float32
     try:
-        if x.dtype is torch.uint8 and w.dtype is torch.uint8 and x_sf.dtype is torch.uint8 and w_sf.dtype is torch.uint8:
-            M, Kb = x.shape
-            N, Kw = w.shape
-            K = 2 * Kb
-            d = x.get_device()
-            if (d >= 0 and Kw == Kb and K and not K % 8 and M and N and x.stride(1) == 1 and w.stride(1) == 1
-                    and w.get_device() == d and x_sf.get_device() == d and w_sf.get_device() == d
-                    and x_sf.dim() == 1 and w_sf.dim() == 1 and x_sf.stride(0) == 1 and w_sf.stride(0) == 1
-                    and x_sf.shape[0] >= _fp4_scale_bytes(M, K, kind) and w_sf.shape[0] >= _fp4_scale_bytes(N, K, kind)
-                    and _vector_ok(x_scale, torch.float32, (M,), d) and _vector_ok(w_scale, torch.float32, (1, N), d)
-                    and _vector_ok(bias, out_dtype, (0, N), d)):
-                return M, N, K, 0 if w_scale is None else w_scale.numel(), 0 if bias is None else bias.numel()
+        M, Kb = x.shape
+        N, Kw = w.shape
+        d = x.get_device()
+        nws = nb = 0
+        ok = (x.dtype is u8 and w.dtype is u8 and x_sf.dtype is u8 and w_sf.dtype is u8 and d >= 0 and Kw == Kb and Kb
+              and not Kb % 4 and M and N and x.stride()[1] == 1 and w.stride()[1] == 1 and w.get_device() == d
+              and x_sf.get_device() == d and w_sf.get_device() == d and x_sf.stride() == (1,) and w_sf.stride() == (1,)
+              and x_sf.numel() >= _fp4_scale_bytes(M, 2 * Kb, kind) and w_sf.numel() >= _fp4_scale_bytes(N, 2 * Kb, kind))
+        if ok and x_scale is not None:
+            ok = (x_scale.dtype is f32 and x_scale.numel() == M and x_scale.get_device() == d and x_scale.is_contiguous())
+        if ok and w_scale is not None:
+            nws = w_scale.numel()
+            ok = w_scale.dtype is f32 and nws in (1, N) and w_scale.get_device() == d and w_scale.is_contiguous()
+        if ok and bias is not None:
+            nb = bias.numel()
+            ok = bias.dtype is out_dtype and nb in (0, N) and bias.get_device() == d and bias.is_contiguous()
+        if ok:
+            return d, M, N, 2 * Kb, nws, nb
     except (AttributeError, TypeError, ValueError, IndexError):
         pass
     return _fp4_product_explain(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype)
@@ -721,7 +728,7 @@ def _fp4_product_explain(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dty
         if nb != N or not bias.is_contiguous():
             raise ValueError("bias must be contiguous with N elements, in the output dtype")
     _one_device(x=x, w=w, x_sf=x_sf, w_sf=w_sf, x_scale=x_scale, w_scale=w_scale, bias=bias if nb else None)
-    return M, N, K, 0 if w_scale is None else w_scale.numel(), nb
+    return x.get_device(), M, N, K, 0 if w_scale is None else w_scale.numel(), nb
 
 
 def _out_matrix(M: int, N: int, dtype: torch.dtype, device) -> torch.Tensor:
@@ -747,7 +754,7 @@ def gemm_fp4(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: torch.T
         out_dtype = out.dtype
     if out_dtype not in OUT_CODE:
         raise TypeError(f"out_dtype {out_dtype} is not one of {tuple(OUT_CODE)}")
-    M, N, K, nws, nb = _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype)
+    d, M, N, K, nws, nb = _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype)
     if out is None:
         out = _out_matrix(M, N, out_dtype, x.device)
     else:
@@ -755,9 +762,10 @@ def gemm_fp4(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: torch.T
         if tuple(out.shape) != (M, N):
             raise ValueError(f"out has shape {tuple(out.shape)}, expected {(M, N)}")
         _one_device(x=x, out=out)
-    _call(_lib.load().t8g_gemm_fp4, x.get_device(), x.data_ptr(), x_sf.data_ptr(), _ptr(x_scale), w.data_ptr(),
-          w_sf.data_ptr(), _ptr(w_scale), nws, bias.data_ptr() if nb else None, nb, out.data_ptr(), OUT_CODE[out_dtype],
-          M, N, K, _pitch(x, 16), _pitch(w, 16), _pitch(out, 16 // out_dtype.itemsize), code, stream)
+    _call(_lib.load().t8g_gemm_fp4, d, x.data_ptr(), x_sf.data_ptr(), None if x_scale is None else x_scale.data_ptr(),
+          w.data_ptr(), w_sf.data_ptr(), None if w_scale is None else w_scale.data_ptr(), nws,
+          bias.data_ptr() if nb else None, nb, out.data_ptr(), OUT_CODE[out_dtype], M, N, K, _pitch(x, M, K // 2, 16),
+          _pitch(w, N, K // 2, 16), _pitch(out, M, N, 16), code, stream)
     return out
 
 
@@ -770,7 +778,7 @@ def gemm_fp4_gated(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: t
     float32 (one rounding, where gemm_gated keeps torch's three), g = gate_index[m] (trusted to be
     rows of gate) or m // rows_per_gate; out may be res itself (in-place update)."""
     code = _fp4_code(kind)
-    M, N, K, nws, nb = _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, torch.bfloat16)
+    idx, M, N, K, nws, nb = _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, torch.bfloat16)
     if gate.dim() == 1:
         gate = gate.view(1, -1)
     if not (res.dtype is torch.bfloat16 and gate.dtype is torch.bfloat16 and res.dim() == 2 and gate.dim() == 2
@@ -801,14 +809,13 @@ def gemm_fp4_gated(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: t
         _need_cuda("out", out, torch.bfloat16, 2)
         if tuple(out.shape) != (M, N):
             raise ValueError(f"out has shape {tuple(out.shape)}, expected {(M, N)}")
-    idx = x.get_device()
     if (res.get_device() != idx or gate.get_device() != idx or out.get_device() != idx
             or (gate_index is not None and gate_index.get_device() != idx)):
         _one_device(x=x, res=res, gate=gate, gate_index=gate_index, out=out)
     _call(_lib.load().t8g_gemm_fp4_gated, idx, x.data_ptr(), x_sf.data_ptr(), _ptr(x_scale), w.data_ptr(),
-          w_sf.data_ptr(), _ptr(w_scale), nws, bias.data_ptr() if nb else None, nb, res.data_ptr(), _pitch(res, 8),
-          gate.data_ptr(), _pitch(gate, 8), _ptr(gate_index), rpg, out.data_ptr(), M, N, K, _pitch(x, 16), _pitch(w, 16),
-          _pitch(out, 8), code, stream)
+          w_sf.data_ptr(), _ptr(w_scale), nws, bias.data_ptr() if nb else None, nb, res.data_ptr(), _pitch(res, M, N, 8),
+          gate.data_ptr(), _pitch(gate, gate.shape[0], N, 8), _ptr(gate_index), rpg, out.data_ptr(), M, N, K,
+          _pitch(x, M, K // 2, 16), _pitch(w, N, K // 2, 16), _pitch(out, M, N, 8), code, stream)
     return out
 
 

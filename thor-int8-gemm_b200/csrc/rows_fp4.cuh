@@ -453,28 +453,33 @@ struct DequantFp4Args {
   int words;
 };
 
+// Thread = one vector of eight columns in the four rows r, r + 32, r + 64, r + 96 of a scale tile, whose scale
+// words are 16 consecutive bytes; the grid's y strides over such groups of rows.
 template <bool MX, int OUT>
 __global__ void __launch_bounds__(256) dequant_rows_fp4_kernel(const DequantFp4Args a) {
-  // thread = one vector of eight; a CTA covers 256 vectors of one row group of rows (gridDim.y strides over rows)
   const int nvec = a.D >> 3;
   const int c = blockIdx.x * blockDim.x + threadIdx.x;
   if (c >= nvec) return;
   const int block = MX ? c >> 2 : c >> 1;
-  const int64_t sf_at = 512 * static_cast<int64_t>(block >> 2) + (block & 3);
-  constexpr int kRows = 4;   // rows in flight per thread
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.y) * kRows; row0 < a.S; row0 += static_cast<int64_t>(gridDim.y) * kRows) {
+  const int64_t groups = (a.S + 127) / 128 * 32;
+  constexpr int kRows = 4;
+  for (int64_t grp = blockIdx.y; grp < groups; grp += gridDim.y) {
+    const int64_t row0 = (grp >> 5) * 128 + (grp & 31);
+    if (row0 >= a.S) continue;
     uint32_t codes[kRows], byte[kRows];
     float rs[kRows];
+    const uint4 words = __ldg(reinterpret_cast<const uint4*>(a.sf + scale_row(row0, a.words) + 512 * static_cast<int64_t>(block >> 2)));
+    const uint32_t w4[kRows] = {words.x, words.y, words.z, words.w};
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const int64_t row = min(row0 + r, a.S - 1);
+      const int64_t row = min(row0 + 32 * r, a.S - 1);
       codes[r] = __ldg(reinterpret_cast<const uint32_t*>(a.q + row * a.ld_q + 4 * static_cast<int64_t>(c)));
-      byte[r] = __ldg(a.sf + scale_row(row, a.words) + sf_at);
+      byte[r] = (w4[r] >> (8 * (block & 3))) & 0xFFu;
       rs[r] = a.q_scale ? __ldg(a.q_scale + row) : 1.f;
     }
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const int64_t row = row0 + r;
+      const int64_t row = row0 + 32 * r;
       if (row >= a.S) break;
       const float sb = MX ? __uint_as_float(byte[r] == 255u ? 0x7FC00000u : byte[r] == 0u ? 0x00400000u : byte[r] << 23)
                           : e4m3_to_f32(byte[r]);

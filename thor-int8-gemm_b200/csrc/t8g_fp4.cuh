@@ -400,9 +400,9 @@ int t8g_dequant_rows_fp4(const void* q, int64_t ld_q, const void* sf, const floa
   a.D = static_cast<int>(D);
   a.words = static_cast<int>(fp4_words(D, quant_kind));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // 256 vectors of four rows a CTA and step; rows are strided over when there are more than the grid holds
+  // 256 vectors of four rows a CTA and step; groups of rows are strided over when the grid holds fewer
   const unsigned gx = static_cast<unsigned>((D / 8 + 255) / 256);
-  const dim3 grid(gx, static_cast<unsigned>(std::min<int64_t>((S + 3) / 4, 65535)));
+  const dim3 grid(gx, static_cast<unsigned>(std::min<int64_t>((S + 127) / 128 * std::min<int64_t>(S, 32), 65535)));
 #define T8G_DEQUANT(MX)                                                                               \
   switch (out_dtype) {                                                                                \
     case T8G_OUT_BF16: dequant_rows_fp4_kernel<MX, 0><<<grid, 256, 0, st>>>(a); break;                \

@@ -56,6 +56,12 @@ def test_scale_bytes_and_rows(kind, s, d):
     assert tiled[at] == byte[r, b]
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_scale_rows_of_nothing(kind):
+    assert ops.fp4_scale_rows(torch.zeros(0, dtype=torch.uint8), 0, 64, kind).shape == (0, 64 // F4.BLOCK[kind])
+    assert ops.fp4_scale_rows(torch.zeros(0, dtype=torch.uint8), 5, 0, kind).shape == (5, 0)
+
+
 def test_scale_bytes_refuses():
     lib = _lib.load()
     assert lib.t8g_fp4_scale_bytes(-1, 64, 2) == -1 and lib.t8g_fp4_scale_bytes(1, 64, 0) == -1

@@ -3,7 +3,8 @@
 Drop-in for the hot path that kylixs/thor-int8-gemm patches into comfy-kitchen:
 the int8 fused-dequant GEMM behind `_C.cutlass_int8_dequant` (plus an fp8 e4m3
 twin), fused RMSNorm + adaLN modulation + quantisation, and fused SwiGLU +
-quantisation.  The kernels are hand-written CUDA for sm_100a behind a C ABI
+quantisation; beside them the same operators in microscaled 4-bit floating point
+(mxfp4, nvfp4).  The kernels are hand-written CUDA for sm_100a behind a C ABI
 (include/thor_int8_gemm_b200.h, libthor_int8_gemm_b200.so next to this file).
 
 Submodules (imported lazily, so the import-proxy agent stays light at start-up):

@@ -519,8 +519,9 @@ def fp4_scale_rows(sf: torch.Tensor, rows: int, D: int, kind: str) -> torch.Tens
     _fp4_code(kind)
     blocks = -(-D // FP4_BLOCK[kind])
     groups = -(-rows // 128)
-    t = sf[:fp4_scale_bytes(rows, D, kind)].view(groups, -(-blocks // 4), 32, 4, 4)
-    return t.permute(0, 3, 2, 1, 4).reshape(groups * 128, -1)[:rows, :blocks]
+    words = -(-blocks // 4)
+    t = sf[:fp4_scale_bytes(rows, D, kind)].view(groups, words, 32, 4, 4)
+    return t.permute(0, 3, 2, 1, 4).reshape(groups * 128, 4 * words)[:rows, :blocks]
 
 
 def _fp4_empty(S: int, D: int, kind: str, device):

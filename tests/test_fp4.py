@@ -155,10 +155,32 @@ def test_cpu_tensors_and_kinds_are_refused():
         ops.dequant_rows_fp4(q, torch.zeros(512, dtype=torch.uint8), None, "mxfp4")
     with pytest.raises(ValueError, match="CUDA"):
         ops.gemm_fp4(q, q, q.view(-1), q.view(-1), kind="mxfp4")
+    with pytest.raises(TypeError, match="torch.Tensor"):
+        ops.gemm_fp4(None, q, q.view(-1), q.view(-1), kind="mxfp4")
     with pytest.raises(TypeError, match="out_dtype"):
         ops.gemm_fp4(q, q, q.view(-1), q.view(-1), kind="mxfp4", out_dtype=torch.float64)
     with pytest.raises(ValueError, match="no 4-bit form"):
         dit.DiTBlock(64, 2, 64, kind="nvfp4", fused_mlp=True)
+
+
+def test_compiled_call_path_declines():
+    """Host tensors, objects that are no tensors, wrong types and shapes are left to the general path,
+    without an exception left behind; a wrong number of arguments is an error."""
+    F = ops._fp4_fast()
+    q, sf, x = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8), torch.zeros(4, 64)
+    out = torch.zeros(4, 4, dtype=torch.bfloat16)
+    assert F.gemm(q, q, sf, sf, None, None, None, out, torch.bfloat16, 0, 8, 2, None) is False
+    assert F.gemm(q, None, 3, sf, None, None, None, out, torch.bfloat16, 0, 8, 2, None) is False
+    assert F.gemm(q, q, sf, sf, None, None, None, out, torch.bfloat16, "0", 8, 2, None) is False
+    assert F.gated(q, q, sf, sf, None, None, None, out, out, out, 4, 2, 0) is False
+    assert F.quant_rows(x, q, sf, None, 2, None) is False
+    assert F.quant_rows("x", q, sf, None, 2, None) is False
+    assert F.swiglu_fc1(x, q, sf, None, 2, None) is False
+    assert F.rms_mod_quant(x, x, x, 4, 0, 1e-6, q, sf, None, 2, None) is False
+    assert F.rms_mod_quant(x, x, x, 4, 0, "eps", q, sf, None, 2, None) is False
+    for f in (F.gemm, F.gated, F.quant_rows, F.swiglu_fc1, F.rms_mod_quant, F.setup):
+        with pytest.raises(TypeError):
+            f(q)
 
 
 @pytest.mark.parametrize("kind", KINDS)

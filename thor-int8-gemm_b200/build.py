@@ -1,6 +1,7 @@
 """Build the C-ABI shared library libthor_int8_gemm_b200.so in place (sm_100a), and the
 small CPython module _t8g_capsule that serves the `_C.cutlass_int8_dequant` proxy straight
-from DLPack capsules (linked against the library, found next to it at run time).
+from DLPack capsules, and _t8g_fp4, the call path of the 4-bit operators (both linked against
+the library, found next to it at run time).
 
     python thor-int8-gemm_b200/build.py [--force]
 
@@ -30,6 +31,8 @@ DEPENDS = SOURCES + [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if 
 
 EXT_SOURCE = os.path.join(CSRC, "capsule.c")
 EXT_PATH = os.path.join(HERE, "_t8g_capsule" + sysconfig.get_config_var("EXT_SUFFIX"))
+FP4_EXT_SOURCE = os.path.join(CSRC, "fp4_call.c")
+FP4_EXT_PATH = os.path.join(HERE, "_t8g_fp4" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -77,24 +80,26 @@ def up_to_date() -> bool:
 
 
 def build_ext(force: bool = False) -> str:
-    """Compile the capsule module (C, against Python's headers and the library)."""
-    deps = [EXT_SOURCE, LIB_PATH, os.path.join(ROOT, "include", "thor_int8_gemm_b200.h")]
-    if not force and os.path.exists(EXT_PATH) and all(os.path.getmtime(p) <= os.path.getmtime(EXT_PATH) for p in deps):
-        return EXT_PATH
-    cc = c_compiler()
-    tmp = EXT_PATH + ".tmp"
-    cmd = [cc, "-O2", "-shared", "-fPIC", "-std=c11", "-I" + sysconfig.get_paths()["include"], "-o", tmp, EXT_SOURCE,
-           "-L" + HERE, "-lthor_int8_gemm_b200", "-Wl,-rpath,$ORIGIN"]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        sys.stderr.write(proc.stdout + proc.stderr)
-        raise RuntimeError(f"building {os.path.basename(EXT_PATH)} failed ({proc.returncode})")
-    os.replace(tmp, EXT_PATH)
+    """Compile the CPython modules (C, against Python's headers and the library); returns the
+    capsule module's path."""
+    for source, path in ((EXT_SOURCE, EXT_PATH), (FP4_EXT_SOURCE, FP4_EXT_PATH)):
+        deps = [source, LIB_PATH, os.path.join(ROOT, "include", "thor_int8_gemm_b200.h")]
+        if not force and os.path.exists(path) and all(os.path.getmtime(p) <= os.path.getmtime(path) for p in deps):
+            continue
+        cc = c_compiler()
+        tmp = path + ".tmp"
+        cmd = [cc, "-O2", "-shared", "-fPIC", "-std=c11", "-I" + sysconfig.get_paths()["include"], "-o", tmp, source,
+               "-L" + HERE, "-lthor_int8_gemm_b200", "-Wl,-rpath,$ORIGIN"]
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            sys.stderr.write(proc.stdout + proc.stderr)
+            raise RuntimeError(f"building {os.path.basename(path)} failed ({proc.returncode})")
+        os.replace(tmp, path)
     return EXT_PATH
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the library (and the capsule module) if any source is newer; return the
+    """Compile the library (and the CPython modules) if any source is newer; return the
     library's path."""
     if not force and up_to_date():
         build_ext()

@@ -99,7 +99,7 @@ def gemm_dequant(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor, w_scal
     float8_e4m3fn (fp32 accumulation); x_scale [M] float32; w_scale [N] or [1]
     float32; bias [N] in the output dtype or None/empty; out [M, N] bf16/fp16/fp32.
     """
-    if out is None and x.dim() == 2 and w.dim() == 2:
+    if out is None and isinstance(x, torch.Tensor) and isinstance(w, torch.Tensor) and x.dim() == 2 and w.dim() == 2:
         out = torch.empty(x.shape[0], w.shape[0], dtype=out_dtype, device=x.device)
     if not _gemm_args_ok(x, w, x_scale, w_scale, bias, out):
         _gemm_args_explain(x, w, x_scale, w_scale, bias, out)
@@ -496,6 +496,33 @@ FP4_CODE = {"mxfp4": _lib.QUANT_MXFP4, "nvfp4": _lib.QUANT_NVFP4}
 FP4_BLOCK = {"mxfp4": 32, "nvfp4": 16}
 
 
+_fp4_module = None
+
+
+def _fp4_fast():
+    """The compiled call path of the common case (csrc/fp4_call.c); each of its functions returns True
+    when it launched, False for the general path below, or the library's status."""
+    global _fp4_module
+    if _fp4_module is None:
+        _lib.load()
+        from . import _t8g_fp4
+        raw = _raw_stream or (lambda idx: torch.cuda.current_stream(idx).cuda_stream)
+        _t8g_fp4.setup(torch.uint8, torch.float32, torch.bfloat16, raw)
+        _fp4_module = _t8g_fp4
+    return _fp4_module
+
+
+def _fp4_launched(r) -> bool:
+    if r is True or r is False:
+        return r
+    _lib.check(r)
+    return True
+
+
+def _raw(stream):
+    return stream if stream is None or isinstance(stream, int) else _stream_handle(None, stream)
+
+
 def _fp4_code(kind: str) -> int:
     if kind not in FP4_CODE:
         raise ValueError(f"kind {kind!r} is not a 4-bit format ({', '.join(FP4_CODE)})")
@@ -587,6 +614,8 @@ def quant_rows_fp4(x: torch.Tensor, kind: str = "nvfp4", stream=None):
     code = _fp4_code(kind)
     S, D = _fp4_bf16_rows("x", x)
     q, sf, q_scale = _fp4_empty(S, D, kind, x.device)
+    if _fp4_launched(_fp4_fast().quant_rows(x, q, sf, q_scale, code, _raw(stream))):
+        return q, sf, q_scale
     idx = x.get_device()
     _call(_lib.load().t8g_quant_rows_fp4, idx, x.data_ptr(), _pitch(x, S, D, 8), q.data_ptr(), _pitch(q, S, D // 2, 16),
           sf.data_ptr(), _ptr(q_scale), S, D, code, stream)
@@ -622,6 +651,11 @@ def rms_mod_quant_fp4(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor,
     bit, without storing h.  Values of mod_index are trusted to be rows of shift / scale."""
     code = _fp4_code(kind)
     S, D = _fp4_bf16_rows("x", x)
+    if w is None and mod_index is None and rows_per_mod:
+        out = _fp4_empty(S, D, kind, x.device)
+        if _fp4_launched(_fp4_fast().rms_mod_quant(x, shift, scale, rows_per_mod, int(scale_is_multiplier), eps, *out, code,
+                                                   _raw(stream))):
+            return out
     idx = x.get_device()
     if not (rows_per_mod and mod_index is None and shift.dim() == 2 and scale.dim() == 2 and shift.shape == scale.shape
             and shift.shape[1] == D and shift.dtype is torch.bfloat16 and scale.dtype is torch.bfloat16
@@ -670,45 +704,20 @@ def swiglu_quant_fp4_fc1(y: torch.Tensor, kind: str = "nvfp4", stream=None):
     M, F2 = _fp4_bf16_rows("y", y)
     if F2 % 16:
         raise ValueError(f"y has rows of {F2} elements: two halves of a multiple of 8 are wanted")
+    out = _fp4_empty(M, F2 // 2, kind, y.device)
+    if _fp4_launched(_fp4_fast().swiglu_fc1(y, *out, _fp4_code(kind), _raw(stream))):
+        return out
     p = y.data_ptr()
     # the up half starts F2 / 2 elements of two bytes in
     return _swiglu_fp4(p, p + F2 if p else p, _pitch(y, M, F2, 8), M, F2 // 2, kind, y.device, stream)
-
-
-def _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype):
-    """Argument rules of the 4-bit products -> (device, M, N, K, w_scale numel, bias numel).  The common
-    case is checked cheaply; anything else goes to _fp4_product_explain, which raises the precise
-    error or accepts the call."""
-    u8, f32 = torch.uint8, torch.float32
-    try:
-        M, Kb = x.shape
-        N, Kw = w.shape
-        d = x.get_device()
-        nws = nb = 0
-        ok = (x.dtype is u8 and w.dtype is u8 and x_sf.dtype is u8 and w_sf.dtype is u8 and d >= 0 and Kw == Kb and Kb
-              and not Kb % 4 and M and N and x.stride()[1] == 1 and w.stride()[1] == 1 and w.get_device() == d
-              and x_sf.get_device() == d and w_sf.get_device() == d and x_sf.stride() == (1,) and w_sf.stride() == (1,)
-              and x_sf.numel() >= _fp4_scale_bytes(M, 2 * Kb, kind) and w_sf.numel() >= _fp4_scale_bytes(N, 2 * Kb, kind))
-        if ok and x_scale is not None:
-            ok = (x_scale.dtype is f32 and x_scale.numel() == M and x_scale.get_device() == d and x_scale.is_contiguous())
-        if ok and w_scale is not None:
-            nws = w_scale.numel()
-            ok = w_scale.dtype is f32 and nws in (1, N) and w_scale.get_device() == d and w_scale.is_contiguous()
-        if ok and bias is not None:
-            nb = bias.numel()
-            ok = bias.dtype is out_dtype and nb in (0, N) and bias.get_device() == d and bias.is_contiguous()
-        if ok:
-            return d, M, N, 2 * Kb, nws, nb
-    except (AttributeError, TypeError, ValueError, IndexError):
-        pass
-    return _fp4_product_explain(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype)
 
 
 def _vector_ok(t, dtype, sizes, device) -> bool:
     return t is None or (t.dtype is dtype and t.numel() in sizes and t.is_contiguous() and t.get_device() == device)
 
 
-def _fp4_product_explain(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype):
+def _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype):
+    """Argument rules of the 4-bit products -> (device, M, N, K, w_scale numel, bias numel)."""
     M, K = _fp4_operand("x", x, x_sf, kind)
     N, Kw = _fp4_operand("w", w, w_sf, kind)
     if Kw != K:
@@ -755,6 +764,13 @@ def gemm_fp4(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: torch.T
         out_dtype = out.dtype
     if out_dtype not in OUT_CODE:
         raise TypeError(f"out_dtype {out_dtype} is not one of {tuple(OUT_CODE)}")
+    fast = out
+    if out is None and isinstance(x, torch.Tensor) and isinstance(w, torch.Tensor) and x.dim() == 2 and w.dim() == 2:
+        fast = out = _out_matrix(x.shape[0], w.shape[0], out_dtype, x.device)
+    if fast is not None and _fp4_launched(_fp4_fast().gemm(x, w, x_sf, w_sf, x_scale, w_scale, bias, out, out_dtype,
+                                                           OUT_CODE[out_dtype], 16 // out_dtype.itemsize, code,
+                                                           _raw(stream))):
+        return out
     d, M, N, K, nws, nb = _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype)
     if out is None:
         out = _out_matrix(M, N, out_dtype, x.device)
@@ -779,6 +795,11 @@ def gemm_fp4_gated(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: t
     float32 (one rounding, where gemm_gated keeps torch's three), g = gate_index[m] (trusted to be
     rows of gate) or m // rows_per_gate; out may be res itself (in-place update)."""
     code = _fp4_code(kind)
+    if rows_per_gate and gate_index is None and isinstance(res, torch.Tensor):
+        to = torch.empty_like(res, memory_format=torch.contiguous_format) if out is None else out
+        if _fp4_launched(_fp4_fast().gated(x, w, x_sf, w_sf, x_scale, w_scale, bias, res, gate, to, rows_per_gate, code,
+                                           _raw(stream))):
+            return to
     idx, M, N, K, nws, nb = _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, torch.bfloat16)
     if gate.dim() == 1:
         gate = gate.view(1, -1)

@@ -236,6 +236,38 @@ def test_wrapper_refusals():
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_general_path_equals_compiled_one(kind, monkeypatch):
+    """What the compiled call path launches, the general one launches too, bit for bit (another stream
+    object, a row map, a wide rows-per-batch count take it anyway)."""
+    class Declines:
+        def __getattr__(self, name):
+            return lambda *a: False
+
+    g = gen(4)
+    m, d, n = 70, 520, 264
+    x, y = randn(g, m, d), randn(g, m, 2 * d)
+    shift, scale = randn(g, 1, d), randn(g, 1, d)
+    w = ops.quant_rows_fp4(randn(g, n, d, scale=0.02), kind)
+    bias, res, gate = randn(g, n), randn(g, m, n), randn(g, 1, n)
+
+    def calls(rows):
+        q = ops.quant_rows_fp4(x, kind)
+        out = [*q, *ops.rms_mod_quant_fp4(x, shift, scale, rows_per_mod=rows, kind=kind),
+               *ops.swiglu_quant_fp4_fc1(y, kind), product(q, w, bias, kind),
+               ops.gemm_fp4_gated(q[0], w[0], q[1], w[1], q[2], w[2], bias, res, gate, rows_per_gate=rows, kind=kind)]
+        # scale tiles hold unwritten rows: compare row by row
+        out[1], out[4], out[7] = (ops.fp4_scale_rows(t, m, d, kind) for t in (out[1], out[4], out[7]))
+        return [t for t in out if t is not None]
+
+    fast = calls(m)
+    wide = calls((1 << 32) + 1)
+    monkeypatch.setattr(ops, "_fp4_module", Declines())
+    general = calls(m)
+    for a, b, c in zip(fast, wide, general):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_offsets_past_2_31(kind):
     """Inputs and outputs of more than 2^31 elements: the last rows equal those of a call of their own."""
     g = gen(2)

@@ -149,7 +149,7 @@ static PyObject* uncommon(void) {
 }
 static int small_int(PyObject* o, int* v) {
   const long x = PyLong_AsLong(o);
-  if (x == -1 && PyErr_Occurred()) return 0;
+  if ((x == -1 && PyErr_Occurred()) || x < INT32_MIN || x > INT32_MAX) return 0;
   *v = (int)x;
   return 1;
 }

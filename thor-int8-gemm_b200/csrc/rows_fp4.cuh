@@ -52,13 +52,6 @@ __device__ __forceinline__ float absmax8(const float2 (&v)[4]) {
   const float b = max3_abs_nan(v[1].y, v[2].x, v[2].y);
   return max3_abs_nan(max3_abs_nan(a, b, v[3].x), v[3].y, 0.f);
 }
-// The same of eight packed bf16 values, as bf16 bits (integer order: NaN above infinity above every
-// number).
-__device__ __forceinline__ uint32_t absmax_bits(const uint4& u) {
-  const uint32_t m = max_u16x2(max_u16x2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu),
-                               max_u16x2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
-  return max(m & 0xFFFFu, m >> 16);
-}
 __device__ __forceinline__ uint32_t warp_max_u32(uint32_t v) {
   uint32_t r;
   asm volatile("redux.sync.max.u32 %0, %1, 0xffffffff;" : "=r"(r) : "r"(v));
@@ -102,18 +95,22 @@ __device__ __forceinline__ float rcp_approx(float v) {   // within 1 ulp; see th
   return r;
 }
 
-// One warp step: lane l holds vector c0 + l of a row (zeros past the row's end).  Returns the eight
-// codes and, in `byte`, the scale of the block that the lane's vector lies in (4 lanes a block for
-// mxfp4, 2 for nvfp4).  Every lane of the warp takes part.
+// A lane's vector c of a row (c % 32 is the lane; vectors of a warp step are consecutive; zeros past the
+// row's end), unpacked: the maximum of the block it lies in (4 lanes a block for mxfp4, 2 for nvfp4;
+// every lane of the warp takes part).
 template <bool MX>
-__device__ __forceinline__ uint32_t quant_vec_fp4(const uint4& u, float row_inverse, uint32_t& byte) {
-  float2 v[4];
-  unpack_pairs(u, v);
-  // magnitudes compare as their bits, NaN above all
-  uint32_t b = __float_as_uint(absmax8(v));
+__device__ __forceinline__ float block_max_fp4(const float2 (&v)[4]) {
+  uint32_t b = __float_as_uint(absmax8(v));   // magnitudes compare as their bits, NaN above all
   b = max(b, __shfl_xor_sync(0xFFFFFFFFu, b, 1));
+  if constexpr (MX) b = max(b, __shfl_xor_sync(0xFFFFFFFFu, b, 2));
+  return __uint_as_float(b);
+}
+
+// The vector's eight codes and its block's scale byte, from the block's maximum.
+template <bool MX>
+__device__ __forceinline__ uint32_t codes_fp4(float2 (&v)[4], float amax, float row_inverse, uint32_t& byte) {
   if constexpr (MX) {
-    b = max(b, __shfl_xor_sync(0xFFFFFFFFu, b, 2));
+    const uint32_t b = __float_as_uint(amax);
     const int e = max(static_cast<int>(b >> 23) - 2, 0);
     const bool finite = b < 0x7F800000u;
     byte = finite ? static_cast<uint32_t>(e) : 255u;
@@ -122,7 +119,7 @@ __device__ __forceinline__ uint32_t quant_vec_fp4(const uint4& u, float row_inve
     for (int p = 0; p < 4; ++p) v[p] = mul2_rn(v[p], make_float2(mult, mult));
   } else {
     // RN(t / 6) with one correction step (quant8 of rows.cuh), then e4m3
-    const float t = __fmul_rn(__uint_as_float(b), row_inverse);
+    const float t = __fmul_rn(amax, row_inverse);
     const float sixth = 1.0f / 6.0f;
     const float q0 = __fmul_rn(t, sixth);
     const float q1 = __fmaf_rn(__fmaf_rn(-6.0f, q0, t), sixth, q0);
@@ -140,26 +137,49 @@ __device__ __forceinline__ uint32_t quant_vec_fp4(const uint4& u, float row_inve
   return cvt_e2m1x8(v);
 }
 
-// Vector c of a row, held in u by lane c % 32 (vectors of a warp step are consecutive): its codes,
-// and its block's scale from the block's first lane.
+// Where a lane's vectors go: the same for every row of a kernel, so kept from row to row.  The vectors are
+// c, c + step, ...; `step` is a multiple of 32, so their scale bytes are equally far apart.
+struct Fp4Lane {
+  int q0, q_step;     // byte of the codes within a row of q
+  int sf0, sf_step;   // byte of the block's scale from the row's first one
+  int steps;          // vectors of the warp: of at least one lane
+  uint32_t codes;     // bit i: vector i exists
+  uint32_t scales;    // bit i: this lane writes vector i's block scale
+};
 template <bool MX>
-__device__ __forceinline__ void store_vec_fp4(uint8_t* qrow, uint8_t* sfrow, int c, int nvec, const uint4& u,
-                                              float row_inverse) {
+__device__ __forceinline__ Fp4Lane fp4_lane(int c, int step, int nvec, int n) {
   constexpr int kLanes = MX ? 4 : 2;   // per block
+  Fp4Lane l;
+  l.q0 = 4 * c;
+  l.q_step = 4 * step;
+  l.sf0 = 512 * (c / (4 * kLanes)) + ((c / kLanes) & 3);
+  l.sf_step = 512 * (step / (4 * kLanes));
+  l.codes = l.scales = 0u;
+  const int first = c & ~31;
+  l.steps = first < nvec ? (nvec - first + step - 1) / step : 0;
+  for (int i = 0; i < n; ++i, c += step) {
+    if (c < nvec) l.codes |= 1u << i;
+    // blocks past the row's last, up to a multiple of four, get the 0 that vectors of zeros have
+    if ((c & (kLanes - 1)) == 0 && (c & ~(4 * kLanes - 1)) < nvec) l.scales |= 1u << i;
+  }
+  return l;
+}
+
+// Codes and scale of a lane's vector i, stored.
+template <bool MX>
+__device__ __forceinline__ void store_vec_fp4(uint8_t* qrow, uint8_t* sfrow, const Fp4Lane& l, int i, float2 (&v)[4],
+                                              float amax, float row_inverse) {
   uint32_t byte;
-  const uint32_t codes = quant_vec_fp4<MX>(u, row_inverse, byte);
-  if (c < nvec) *reinterpret_cast<uint32_t*>(qrow + 4 * c) = codes;
-  // blocks past the row's last, up to a multiple of four, get the 0 that vectors of zeros have
-  if ((c & (kLanes - 1)) == 0 && (c & ~(4 * kLanes - 1)) < nvec)
-    sfrow[512 * (c / (4 * kLanes)) + ((c / kLanes) & 3)] = static_cast<uint8_t>(byte);
+  const uint32_t codes = codes_fp4<MX>(v, amax, row_inverse, byte);
+  if (l.codes >> i & 1u) *reinterpret_cast<uint32_t*>(qrow + l.q0 + i * l.q_step) = codes;
+  if (l.scales >> i & 1u) sfrow[l.sf0 + i * l.sf_step] = static_cast<uint8_t>(byte);
 }
 
 // ---------------------------------------------------------------- direct row kernels
 // Quantisation and norm: a row group of T threads per row with its V vectors a thread in registers
-// (thread t holds vectors t, t + T, ...), loaded straight from global memory while the row before is
-// worked on; a CTA holds as many groups as make 256 threads.  A group owns consecutive rows, so it
-// keeps the modulation in registers until the batch element changes.  No ring and no set-up: a
-// single row takes one round trip to memory.  (T, V) is the canonical row-group shape, which makes
+// (thread t holds vectors t, t + T, ...), loaded straight from global memory (quantisation: while the row
+// before is worked on); a CTA holds as many groups as make 256 threads, a group takes consecutive
+// rows.  No ring and no set-up: a single row takes one round trip to memory.  (T, V) is the canonical row-group shape, which makes
 // the norm's sum of squares the 8-bit kernels', bit for bit.
 __device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
   uint4 v;
@@ -179,24 +199,35 @@ __device__ __forceinline__ uint32_t group_max_u32(const RowGroup& grp, uint32_t 
   return warp_max_u32(lane < (grp.T >> 5) ? __float_as_uint(red[lane]) : 0u);
 }
 
-// Quantises the V vectors a thread of the group holds (zeros past the row's end).
+// Quantises the V vectors a thread of the group holds (zeros past the row's end).  The row's maximum
+// comes from the block maxima, which the scales need anyway.
 template <bool MX, int V>
-__device__ __forceinline__ void group_quant_fp4(const RowGroup& grp, const Fp4Out& o, int64_t row, const uint4 (&v)[V],
-                                                int nvec, float* red) {
+__device__ __forceinline__ void group_quant_fp4(const RowGroup& grp, const Fp4Out& o, int64_t row, const uint4 (&u)[V],
+                                                const Fp4Lane& lane, float* red) {
+  uint8_t* qrow = o.q + row * o.ld_q;
+  uint8_t* sfrow = o.sf + scale_row(row, o.words);
+  float top[V];
   float inverse = 0.f;
   if constexpr (!MX) {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) m = max(m, absmax_bits(v[i]));
-    const float scale = row_scale_fp4(group_max_u32(grp, m, red), &inverse);
+    for (int i = 0; i < V; ++i) {
+      if (i >= lane.steps) break;
+      float2 v[4];
+      unpack_pairs(u[i], v);
+      top[i] = block_max_fp4<MX>(v);
+      m = max(m, __float_as_uint(top[i]));
+    }
+    const float scale = row_scale_fp4(group_max_u32(grp, m, red) >> 16, &inverse);   // bf16 values: low half 0, or NaN
     if (grp.t == 0) o.q_scale[row] = scale;
   }
-  uint8_t* qrow = o.q + row * o.ld_q;
-  uint8_t* sfrow = o.sf + scale_row(row, o.words);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int c = grp.t + grp.T * i;
-    if (c - (grp.t & 31) < nvec) store_vec_fp4<MX>(qrow, sfrow, c, nvec, v[i], inverse);   // warp-uniform
+    if (i >= lane.steps) break;
+    float2 v[4];
+    unpack_pairs(u[i], v);
+    if constexpr (MX) top[i] = block_max_fp4<MX>(v);
+    store_vec_fp4<MX>(qrow, sfrow, lane, i, v, top[i], inverse);
   }
 }
 
@@ -212,8 +243,10 @@ __device__ __forceinline__ void load_row_fp4(uint4 (&v)[V], const __nv_bfloat16*
 enum Fp4Source : int { kFp4Plain = 0, kFp4Norm = 1, kFp4NormWeight = 2 };
 
 // rows_per_group rows for each group; a holds x (and, for the norm, its operands).
+// Three vectors a thread keep to 64 registers, so that two of the widest CTAs share an SM: with the next row
+// and the modulation held in registers the norm had one, and 8192 x 8192 mxfp4 took 96 us (now 81).
 template <bool MX, int V, int SRC>
-__global__ void __launch_bounds__(512) rows_fp4_kernel(const RmsArgs a, const Fp4Out o, const int T,
+__global__ void __launch_bounds__(512, V == 3 ? 2 : 1) rows_fp4_kernel(const RmsArgs a, const Fp4Out o, const int T,
                                                        const int64_t rows_per_group) {
   // two of each, used by rows in turn: a warp may write the next row's partials while another still
   // reads this row's, and the next row's barrier lies between this row's reads and the one after's writes
@@ -225,42 +258,15 @@ __global__ void __launch_bounds__(512) rows_fp4_kernel(const RmsArgs a, const Fp
   const int64_t first = (static_cast<int64_t>(blockIdx.x) * grp.count + grp.index) * rows_per_group;
   const int64_t end = min(first + rows_per_group, a.S);
   if (first >= end) return;   // a whole group leaves: its barriers are its own
-  uint4 v[V], next[V];
+  const Fp4Lane where = fp4_lane<MX>(grp.t, T, nvec, V);
+  uint4 v[V];
+  [[maybe_unused]] uint4 next[SRC == kFp4Plain ? V : 1];
   load_row_fp4<V>(v, a.x + first * a.ld_x, grp.t, T, nvec);
-  [[maybe_unused]] uint4 mul[SRC ? V : 1], shift[SRC ? V : 1], weight[SRC == kFp4NormWeight ? V : 1];
-  [[maybe_unused]] int64_t cur = -1, seg_end = -1;
-  if constexpr (SRC == kFp4NormWeight) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = grp.t + T * i;
-      weight[i] = c < nvec ? ld_v4(a.w + 8 * c) : make_uint4(0, 0, 0, 0);
-    }
-  }
   for (int64_t row = first; row < end; ++row) {
-    if (row + 1 < end) load_row_fp4<V>(next, a.x + (row + 1) * a.ld_x, grp.t, T, nvec);
-    if constexpr (SRC != kFp4Plain) {
-      int64_t m = cur;
-      if (a.mod_index) {
-        m = static_cast<int64_t>(__ldg(a.mod_index + row));
-      } else if (row >= seg_end) {
-        m = row / a.rows_per_mod;
-        seg_end = (m + 1) * a.rows_per_mod;
-      }
-      if (m != cur) {   // the same for the whole group
-        cur = m;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int c = grp.t + T * i;
-          mul[i] = shift[i] = make_uint4(0, 0, 0, 0);
-          if (c < nvec) {
-            mul[i] = ld_v4(a.scale + m * a.ld_mod + 8 * c);
-            shift[i] = ld_v4(a.shift + m * a.ld_mod + 8 * c);
-          }
-          if (!a.scale_is_multiplier)
-            mul[i] = make_uint4(one_plus_bf16x2(mul[i].x), one_plus_bf16x2(mul[i].y), one_plus_bf16x2(mul[i].z),
-                                one_plus_bf16x2(mul[i].w));
-        }
-      }
+    if constexpr (SRC == kFp4Plain) {
+      if (row + 1 < end) load_row_fp4<V>(next, a.x + (row + 1) * a.ld_x, grp.t, T, nvec);
+    } else {
+      const int64_t m = a.mod_index ? static_cast<int64_t>(__ldg(a.mod_index + row)) : row / a.rows_per_mod;
       // vectors past the row's end are zeros and leave the sums as they are
       float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
@@ -275,27 +281,36 @@ __global__ void __launch_bounds__(512) rows_fp4_kernel(const RmsArgs a, const Fp
       const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
+        const int c = grp.t + T * i;
+        if (c >= nvec) continue;   // stays zero
+        uint4 su = ld_v4(a.scale + m * a.ld_mod + 8 * c);
+        if (!a.scale_is_multiplier)
+          su = make_uint4(one_plus_bf16x2(su.x), one_plus_bf16x2(su.y), one_plus_bf16x2(su.z), one_plus_bf16x2(su.w));
+        const uint4 bu = ld_v4(a.shift + m * a.ld_mod + 8 * c);
+        uint4 wu = make_uint4(0, 0, 0, 0);
+        if constexpr (SRC == kFp4NormWeight) wu = ld_v4(a.w + 8 * c);
         const uint32_t xw[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-        const uint32_t sw[4] = {mul[i].x, mul[i].y, mul[i].z, mul[i].w};
-        const uint32_t bw[4] = {shift[i].x, shift[i].y, shift[i].z, shift[i].w};
+        const uint32_t sw[4] = {su.x, su.y, su.z, su.w};
+        const uint32_t bw[4] = {bu.x, bu.y, bu.z, bu.w};
+        const uint32_t ww[4] = {wu.x, wu.y, wu.z, wu.w};
         uint32_t h[4];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
           float2 t = mul2_rn(bf2_to_f2(xw[p]), inv2);
-          if constexpr (SRC == kFp4NormWeight) {
-            const uint32_t ww[4] = {weight[i].x, weight[i].y, weight[i].z, weight[i].w};
-            t = mul2_rn(t, bf2_to_f2(ww[p]));
-          }
+          if constexpr (SRC == kFp4NormWeight) t = mul2_rn(t, bf2_to_f2(ww[p]));
           h[p] = f2_to_bf2(add_f32_bf16x2(mul2_rn(t, bf2_to_f2(sw[p])), bw[p]));
         }
         v[i] = make_uint4(h[0], h[1], h[2], h[3]);
-        if (grp.t + T * i >= nvec) v[i] = make_uint4(0, 0, 0, 0);   // 0 times an infinite inv
       }
     }
-    group_quant_fp4<MX, V>(grp, o, row, v, nvec, red_max[turn] + grp.index * (T >> 5));
+    group_quant_fp4<MX, V>(grp, o, row, v, where, red_max[turn] + grp.index * (T >> 5));
     turn ^= 1;
+    if constexpr (SRC == kFp4Plain) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = next[i];
+      for (int i = 0; i < V; ++i) v[i] = next[i];
+    } else {
+      if (row + 1 < end) load_row_fp4<V>(v, a.x + (row + 1) * a.ld_x, grp.t, T, nvec);
+    }
   }
 }
 
@@ -353,6 +368,10 @@ __global__ void __launch_bounds__(32 * kFp4NormWarps, 1)
   float4* cache = mod_cache_of<NV>(smem, g);
   const int64_t cm = fill_mod_cache<NV, HAS_W>(a, g, cache);
   __syncthreads();
+  constexpr uint32_t kAll = (1u << NV) - 1u;   // every vector of the row exists
+  Fp4Lane where = fp4_lane<MX>(lane, 32, 32 * NV, 0);
+  where.codes = kAll;
+  where.scales = (lane & (MX ? 3 : 1)) == 0 ? kAll : 0u;
   int64_t cur_m = -1, seg_end = -1;
   auto src = [&](int64_t r) -> const void* { return a.x + r * a.ld_x; };
   warp_row_loop_reg(
@@ -392,7 +411,11 @@ __global__ void __launch_bounds__(32 * kFp4NormWarps, 1)
         uint8_t* qrow = o.q + row * o.ld_q;
         uint8_t* sfrow = o.sf + scale_row(row, o.words);
 #pragma unroll
-        for (int k = 0; k < NV; ++k) store_vec_fp4<MX>(qrow, sfrow, 32 * k + lane, 32 * NV, r.v[k], inverse);
+        for (int k = 0; k < NV; ++k) {
+          float2 v[4];
+          unpack_pairs(r.v[k], v);
+          store_vec_fp4<MX>(qrow, sfrow, where, k, v, block_max_fp4<MX>(v), inverse);
+        }
       });
 }
 
@@ -409,6 +432,7 @@ __global__ void __launch_bounds__(1024) swiglu_fp4_kernel(const SwigluArgs a, co
   const RowGroup grp = row_group(T);
   uint8_t* ring = smem + kSigmoidBytes + static_cast<size_t>(grp.index) * ring_bytes(g);
   const int nvec = a.F >> 3;
+  const Fp4Lane where = fp4_lane<MX>(grp.t, T, nvec, V);
   auto src = [&](int64_t r, int part) -> const void* { return (part ? a.up : a.gate) + r * a.ld_in; };
   row_loop(ring, g, grp, a.M, src, [&](int64_t row, uint8_t* slot, const RingState& rs) {
     const uint8_t* up = slot + g.part_bytes;
@@ -419,7 +443,7 @@ __global__ void __launch_bounds__(1024) swiglu_fp4_kernel(const SwigluArgs a, co
       const int c = grp.t + T * i;
       v[i] = c < nvec ? swiglu8(slot, up, c, sig, unused, false) : make_uint4(0, 0, 0, 0);
     }
-    group_quant_fp4<MX, V>(grp, o, row, v, nvec, rs.red_max);
+    group_quant_fp4<MX, V>(grp, o, row, v, where, rs.red_max);
   });
 }
 

@@ -51,12 +51,11 @@ struct StageDescs {
   uint64_t a, b, sfa, sfb;
 };
 
-// MMAs of one stage, issued by one elected lane: copy its scales to TMEM, then `steps` K = 64
+// One stage's work of the MMA warp, issued by one elected lane: its scales to TMEM, then STEPS K = 64
 // products.  `sa_t` / `sb_t`: TMEM columns of A's scales (4 per tile) and B's (4 * B_GROUPS per
 // tile), B's moved by `sb_off` to this output tile's rows.
 template <bool MX, bool PAIR, int B_GROUPS, int STEPS>
-__device__ __forceinline__ void stage_mmas_n(uint32_t d_tmem, const StageDescs& d, uint32_t sa_t, uint32_t sb_t,
-                                             uint32_t sb_off, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void stage_scales_n(const StageDescs& d, uint32_t sa_t, uint32_t sb_t) {
   constexpr int kTiles = stage_tiles(MX);
   constexpr int kUsed = MX ? (STEPS + 1) / 2 : STEPS;
 #pragma unroll
@@ -66,6 +65,10 @@ __device__ __forceinline__ void stage_mmas_n(uint32_t d_tmem, const StageDescs& 
     for (int g = 0; g < B_GROUPS; ++g)
       tmem_cp_scales<PAIR>(sb_t + 4u * (B_GROUPS * t + g), d.sfb + (g * kTiles + t) * (kScaleTile / 16));
   }
+}
+template <bool MX, bool PAIR, int B_GROUPS, int STEPS>
+__device__ __forceinline__ void stage_products_n(uint32_t d_tmem, const StageDescs& d, uint32_t sa_t, uint32_t sb_t,
+                                                 uint32_t sb_off, uint32_t idesc, uint32_t accumulate) {
 #pragma unroll
   for (int k = 0; k < STEPS; ++k) {
     const uint32_t t = MX ? k >> 1 : k;
@@ -78,14 +81,19 @@ __device__ __forceinline__ void stage_mmas_n(uint32_t d_tmem, const StageDescs& 
 template <bool MX, bool PAIR, int B_GROUPS>
 __device__ __forceinline__ void stage_mmas(uint32_t d_tmem, const StageDescs& d, uint32_t sa_t, uint32_t sb_t,
                                            uint32_t sb_off, uint32_t idesc, int steps, uint32_t accumulate) {
-  if (steps == 4)
-    stage_mmas_n<MX, PAIR, B_GROUPS, 4>(d_tmem, d, sa_t, sb_t, sb_off, idesc, accumulate);
-  else if (steps == 3)
-    stage_mmas_n<MX, PAIR, B_GROUPS, 3>(d_tmem, d, sa_t, sb_t, sb_off, idesc, accumulate);
-  else if (steps == 2)
-    stage_mmas_n<MX, PAIR, B_GROUPS, 2>(d_tmem, d, sa_t, sb_t, sb_off, idesc, accumulate);
-  else
-    stage_mmas_n<MX, PAIR, B_GROUPS, 1>(d_tmem, d, sa_t, sb_t, sb_off, idesc, accumulate);
+#define T8G_STAGE(STEPS)                                                                            \
+  stage_scales_n<MX, PAIR, B_GROUPS, STEPS>(d, sa_t, sb_t);                                         \
+  stage_products_n<MX, PAIR, B_GROUPS, STEPS>(d_tmem, d, sa_t, sb_t, sb_off, idesc, accumulate)
+  if (steps == 4) {
+    T8G_STAGE(4);
+  } else if (steps == 3) {
+    T8G_STAGE(3);
+  } else if (steps == 2) {
+    T8G_STAGE(2);
+  } else {
+    T8G_STAGE(1);
+  }
+#undef T8G_STAGE
 }
 
 // ---------------------------------------------------------------- 1-SM kernel
@@ -676,13 +684,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       uint32_t phase = 0;
       bool ok = true, any = false;
       for (int tile = pair; ok && tile < num_tiles; tile += npairs, ++local) {
-        // the shared columns of the tile before; the other columns of this accumulator were read
-        // before that tile's epilogue began (every warp reports)
-        if (local > 0 && !mbar_wait_warp(&s.shared_free, static_cast<uint32_t>(local - 1) & 1u, kStatusTimeoutMma)) break;
-        tc_fence_after();
         const int acc = local & 1;
         const uint32_t d_tmem = tmem_base + (acc ? 256u - C::kOver : 0u);
-        for (int kb = 0; kb < args.kstages; ++kb) {
+        int kb = 0;
+        if (local > 0 && args.kstages > 1) {
+          // The first stage's scales go to TMEM while the tile before still hands over the columns its
+          // accumulator shares with this one.  (Its other columns were read before that tile's
+          // epilogue began: every warp reports.)
+          if (!mbar_wait_warp(&s.full[stage], phase, kStatusTimeoutMma)) break;
+          tc_fence_after();
+          const StageDescs d = {d0.a + stage * (C::kABytes / 16), d0.b + stage * (C::kBBytes / 16),
+                                d0.sfa + stage * (C::kSfaBytes / 16), d0.sfb + stage * (C::kSfbBytes / 16)};
+          if (elect_one()) stage_scales_n<MX, true, 2, 4>(d, sa_t, sb_t);
+          __syncwarp();
+          if (!mbar_wait_warp(&s.shared_free, static_cast<uint32_t>(local - 1) & 1u, kStatusTimeoutMma)) break;
+          tc_fence_after();
+          if (elect_one()) {
+            stage_products_n<MX, true, 2, 4>(d_tmem, d, sa_t, sb_t, 0u, idesc, 0u);
+            tc_commit_both(smem_u32(&s.empty[stage]));
+          }
+          __syncwarp();
+          if (++stage == C::kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          kb = 1;
+        } else if (local > 0) {
+          if (!mbar_wait_warp(&s.shared_free, static_cast<uint32_t>(local - 1) & 1u, kStatusTimeoutMma)) break;
+          tc_fence_after();
+        }
+        for (; kb < args.kstages; ++kb) {
           if (!mbar_wait_warp(&s.full[stage], phase, kStatusTimeoutMma)) {
             ok = false;
             break;

@@ -173,12 +173,13 @@ def test_compiled_call_path_declines():
     assert F.gemm(q, None, 3, sf, None, None, None, out, torch.bfloat16, 0, 8, 2, None) is False
     assert F.gemm(q, q, sf, sf, None, None, None, out, torch.bfloat16, "0", 8, 2, None) is False
     assert F.gated(q, q, sf, sf, None, None, None, out, out, out, 4, 2, 0) is False
+    assert F.dequant(q, sf, None, x, 2, 2, None) is False
     assert F.quant_rows(x, q, sf, None, 2, None) is False
     assert F.quant_rows("x", q, sf, None, 2, None) is False
     assert F.swiglu_fc1(x, q, sf, None, 2, None) is False
     assert F.rms_mod_quant(x, x, x, 4, 0, 1e-6, q, sf, None, 2, None) is False
     assert F.rms_mod_quant(x, x, x, 4, 0, "eps", q, sf, None, 2, None) is False
-    for f in (F.gemm, F.gated, F.quant_rows, F.swiglu_fc1, F.rms_mod_quant, F.setup):
+    for f in (F.gemm, F.gated, F.dequant, F.quant_rows, F.swiglu_fc1, F.rms_mod_quant, F.setup):
         with pytest.raises(TypeError):
             f(q)
 

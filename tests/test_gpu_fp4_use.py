@@ -253,7 +253,7 @@ def test_general_path_equals_compiled_one(kind, monkeypatch):
     def calls(rows):
         q = ops.quant_rows_fp4(x, kind)
         out = [*q, *ops.rms_mod_quant_fp4(x, shift, scale, rows_per_mod=rows, kind=kind),
-               *ops.swiglu_quant_fp4_fc1(y, kind), product(q, w, bias, kind),
+               *ops.swiglu_quant_fp4_fc1(y, kind), product(q, w, bias, kind), ops.dequant_rows_fp4(*q, kind),
                ops.gemm_fp4_gated(q[0], w[0], q[1], w[1], q[2], w[2], bias, res, gate, rows_per_gate=rows, kind=kind)]
         # scale tiles hold unwritten rows: compare row by row
         out[1], out[4], out[7] = (ops.fp4_scale_rows(t, m, d, kind) for t in (out[1], out[4], out[7]))

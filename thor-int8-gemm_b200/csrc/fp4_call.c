@@ -286,6 +286,29 @@ static PyObject* rms_mod_quant(PyObject* self, PyObject* const* a, Py_ssize_t n)
   return result(rc);
 }
 
+/* dequant(q, sf, q_scale, out, out_code, kind, stream): out [S, D], contiguous, just allocated by the caller */
+static PyObject* dequant(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  Matrix q;
+  int64_t dev, n_scale;
+  void *sf, *scale, *out, *stream;
+  int out_code, kind;
+  if (n != 7 || !t_u8) {
+    PyErr_SetString(PyExc_TypeError, "dequant: 7 arguments, after setup()");
+    return NULL;
+  }
+  if (!small_int(a[4], &out_code) || !small_int(a[5], &kind) || !current_device_of(a[0], &dev) ||
+      !matrix(a[0], t_u8, 16, &q) || q.cols % 4 || !scales(a[1], t8g_fp4_scale_bytes(q.rows, 2 * q.cols, kind), dev, &sf) ||
+      !vector(a[2], t_f32, q.rows, q.rows, dev, &scale, &n_scale) || !device_is(a[3], dev) || !address(a[3], &out) ||
+      !stream_of(a[6], dev, &stream))
+    return uncommon();
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = t8g_dequant_rows_fp4(q.p, q.ld, sf, (const float*)scale, out, out_code, 2 * q.cols, q.rows, 2 * q.cols, kind, stream);
+  Py_END_ALLOW_THREADS
+  return result(rc);
+}
+
 /* setup(torch.uint8, torch.float32, torch.bfloat16, raw_stream) */
 static PyObject* setup(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   (void)self;
@@ -308,6 +331,7 @@ static PyMethodDef methods[] = {{"setup", FAST(setup), "Keep torch's dtype objec
                                 {"quant_rows", FAST(quant_rows), "t8g_quant_rows_fp4, the common case."},
                                 {"swiglu_fc1", FAST(swiglu_fc1), "t8g_swiglu_quant_fp4 of an fc1 output, the common case."},
                                 {"rms_mod_quant", FAST(rms_mod_quant), "t8g_rms_mod_quant_fp4, the common case."},
+                                {"dequant", FAST(dequant), "t8g_dequant_rows_fp4, the common case."},
                                 {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_t8g_fp4", NULL, -1, methods};
 

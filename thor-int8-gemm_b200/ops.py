@@ -612,10 +612,12 @@ def quant_rows_fp4(x: torch.Tensor, kind: str = "nvfp4", stream=None):
     e4m3 scale, and a power of two per row.  A block (mxfp4) or row (nvfp4) that holds a NaN or an
     infinity stands for NaN."""
     code = _fp4_code(kind)
+    if isinstance(x, torch.Tensor) and x.dim() == 2:
+        out = _fp4_empty(*x.shape, kind, x.device)
+        if _fp4_launched(_fp4_fast().quant_rows(x, *out, code, _raw(stream))):
+            return out
     S, D = _fp4_bf16_rows("x", x)
     q, sf, q_scale = _fp4_empty(S, D, kind, x.device)
-    if _fp4_launched(_fp4_fast().quant_rows(x, q, sf, q_scale, code, _raw(stream))):
-        return q, sf, q_scale
     idx = x.get_device()
     _call(_lib.load().t8g_quant_rows_fp4, idx, x.data_ptr(), _pitch(x, S, D, 8), q.data_ptr(), _pitch(q, S, D // 2, 16),
           sf.data_ptr(), _ptr(q_scale), S, D, code, stream)
@@ -626,6 +628,12 @@ def dequant_rows_fp4(q: torch.Tensor, sf: torch.Tensor, q_scale: torch.Tensor | 
                      out_dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
     """What a 4-bit matrix stands for: (code * block scale) * q_scale as bf16, fp16 or fp32 [S, D]."""
     code = _fp4_code(kind)
+    if out_dtype not in OUT_CODE:
+        raise TypeError(f"out_dtype {out_dtype} is not one of {tuple(OUT_CODE)}")
+    if isinstance(q, torch.Tensor) and q.dim() == 2:
+        out = torch.empty(q.shape[0], 2 * q.shape[1], dtype=out_dtype, device=q.device)
+        if _fp4_launched(_fp4_fast().dequant(q, sf, q_scale, out, OUT_CODE[out_dtype], code, _raw(stream))):
+            return out
     S, D = _fp4_operand("q", q, sf, kind)
     if D % 8:
         raise ValueError(f"q has rows of {D} elements, not a multiple of 8")
@@ -634,8 +642,6 @@ def dequant_rows_fp4(q: torch.Tensor, sf: torch.Tensor, q_scale: torch.Tensor | 
         _need_cuda("q_scale", q_scale, torch.float32, 1)
         if q_scale.numel() != S or not q_scale.is_contiguous():
             raise ValueError("q_scale must be a contiguous float32 tensor with S elements")
-    if out_dtype not in OUT_CODE:
-        raise TypeError(f"out_dtype {out_dtype} is not one of {tuple(OUT_CODE)}")
     if sf.get_device() != idx or (q_scale is not None and q_scale.get_device() != idx):
         _one_device(q=q, sf=sf, q_scale=q_scale)
     out = torch.empty(S, D, dtype=out_dtype, device=q.device)
@@ -650,12 +656,12 @@ def rms_mod_quant_fp4(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor,
     """rms_mod_quant with 4-bit output -> (q, sf, q_scale): quant_rows_fp4 of its bf16 h, bit for
     bit, without storing h.  Values of mod_index are trusted to be rows of shift / scale."""
     code = _fp4_code(kind)
-    S, D = _fp4_bf16_rows("x", x)
-    if w is None and mod_index is None and rows_per_mod:
-        out = _fp4_empty(S, D, kind, x.device)
+    if w is None and mod_index is None and rows_per_mod and isinstance(x, torch.Tensor) and x.dim() == 2:
+        out = _fp4_empty(*x.shape, kind, x.device)
         if _fp4_launched(_fp4_fast().rms_mod_quant(x, shift, scale, rows_per_mod, int(scale_is_multiplier), eps, *out, code,
                                                    _raw(stream))):
             return out
+    S, D = _fp4_bf16_rows("x", x)
     idx = x.get_device()
     if not (rows_per_mod and mod_index is None and shift.dim() == 2 and scale.dim() == 2 and shift.shape == scale.shape
             and shift.shape[1] == D and shift.dtype is torch.bfloat16 and scale.dtype is torch.bfloat16
@@ -701,12 +707,14 @@ def _swiglu_fp4(gate: int, up: int, ld: int, M: int, F: int, kind: str, device, 
 
 def swiglu_quant_fp4_fc1(y: torch.Tensor, kind: str = "nvfp4", stream=None):
     """swiglu_quant_fp4 of a [M, 2F] fc1 output whose first half is the gate (read in place)."""
+    code = _fp4_code(kind)
+    if isinstance(y, torch.Tensor) and y.dim() == 2:
+        out = _fp4_empty(y.shape[0], y.shape[1] // 2, kind, y.device)
+        if _fp4_launched(_fp4_fast().swiglu_fc1(y, *out, code, _raw(stream))):
+            return out
     M, F2 = _fp4_bf16_rows("y", y)
     if F2 % 16:
         raise ValueError(f"y has rows of {F2} elements: two halves of a multiple of 8 are wanted")
-    out = _fp4_empty(M, F2 // 2, kind, y.device)
-    if _fp4_launched(_fp4_fast().swiglu_fc1(y, *out, _fp4_code(kind), _raw(stream))):
-        return out
     p = y.data_ptr()
     # the up half starts F2 / 2 elements of two bytes in
     return _swiglu_fp4(p, p + F2 if p else p, _pitch(y, M, F2, 8), M, F2 // 2, kind, y.device, stream)

@@ -23,7 +23,6 @@ namespace gemm4 {
 
 using gemm::BK;
 using gemm::BM;
-using gemm::EPI_COLS;
 using gemm::kOutBF16;
 using gemm::kOutF16;
 using gemm::kOutF32;
@@ -352,8 +351,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
 // overlap, but feed the tensor cores 14 % more operand bytes per product.)
 // A CTA needs its own 128 rows' scales of A but those of all 256 rows of W: both CTAs load them.
 //
-// Eight epilogue warps (four would take 4.6 us a tile, more than the 3.2 us that its MMAs take at K = 3072):
-// warp 2 + 4 h + i reads the 32 lanes 32 ((2 + i) % 4) .. of columns [128 h, 128 h + 128).
+// Eight epilogue warps share a CTA's half of a tile: warp 2 + 4 h + i reads the 32 lanes 32 ((2 + i) % 4) .. of columns [128 h, 128 h + 128).
 constexpr int kEpiWarps = 8;
 constexpr int kPairThreads = 64 + 32 * kEpiWarps;
 constexpr int kHalfCols = gemm::BN / 2;

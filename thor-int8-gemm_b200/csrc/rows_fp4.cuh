@@ -1,4 +1,4 @@
-// Row kernels of the microscaled 4-bit formats (HBM-bound): quantisation of bf16 rows, RMSNorm +
+// Row kernels of the microscaled 4-bit formats (bound by HBM and instruction issue): quantisation of bf16 rows, RMSNorm +
 // modulation + quantisation, SwiGLU + quantisation, and the inverse.
 //
 // e2m1 values 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign, rounded to nearest (ties to the even

@@ -168,6 +168,29 @@ def test_padding_is_not_read_into_results(kind, m, n, k):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,n,k", [(4921, 4112, 8), (4921, 4112, 520), (2305, 9232, 264)])
+def test_tiles_without_work_for_some_warps(kind, m, n, k):
+    """Persistent tiles where some epilogue warps have no rows or no columns and run ahead of the others: the
+    result does not depend on which warp is first."""
+    g = gen(m + n)
+    x, w = ops.quant_rows_fp4(randn(g, m, k), kind), ops.quant_rows_fp4(randn(g, n, k, scale=0.02), kind)
+    res, gate = randn(g, m, n), randn(g, 3, n)
+    val = lambda o: ops.dequant_rows_fp4(*o, kind, out_dtype=torch.float32).double()  # noqa: E731
+    y = val(x) @ val(w).t()
+    rows = -(-m // 3)
+    want = res.double() + gate.double()[torch.arange(m, device=DEV) // rows] * y
+    first = None
+    for _ in range(8):
+        got = ops.gemm_fp4_gated(x[0], w[0], x[1], w[1], x[2], w[2], None, res, gate, rows_per_gate=rows, kind=kind)
+        # half a bf16 unit, and float32 accumulation far below 2^-14 of these operands' sums
+        assert ((got.double() - want).abs() <= want.abs() * 2.0 ** -8 + 2.0 ** -14 * y.abs().max()).all()
+        out = product(x, w, kind=kind)
+        assert ((out.double() - y).abs() <= y.abs() * 2.0 ** -8 + 2.0 ** -14 * y.abs().max()).all()
+        first = first or (got, out)
+        assert torch.equal(got, first[0]) and torch.equal(out, first[1])
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_scales_and_repeats(kind):
     """Row and weight scales in their forms (a row, one for all, none), an operand without a row scale,
     and the same bits from the same call, with K split over a cluster and not."""

@@ -755,10 +755,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const int acc = local & 1;
       const int row0 = tm * P_BM + rank * 128 + quarter * 32;
       const int n0 = tn * BN + half * kHalfCols;
-      // the shared columns are the upper half's of accumulator 0 and the lower half's of 1; the other
-      // half (and a warp without rows) only reports that it is done with the tile before
+      // the shared columns are the upper half's of accumulator 0 and the lower half's of 1
       const bool shared = row0 < args.M && half != acc;
-      if (!shared && lane == 0) mbar_arrive_cluster_relaxed(shared_bar);
       stage_params<OUT>(args, tn * BN, e, s.params[acc]);
       const float xs_r = (row0 + lane < args.M && args.xs) ? __ldg(args.xs + row0 + lane) : 1.f;
       GatedSlice gs{};
@@ -769,6 +767,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       if (named_bar_any(1, 32 * kEpiWarps, !ok)) break;
       ok = mbar_wait_warp(&s.tmem_full[acc], static_cast<uint32_t>((local >> 1) & 1), kStatusTimeoutEpilogue);
       tc_fence_after();
+      // The other half, and a warp without rows, report as well, which tells that they are done with the tile
+      // before.  Only now: this tile's MMAs began when the tile before had all its reports, so no warp's
+      // report for this tile can be taken for a slower warp's for that one.
+      if (ok && !shared && lane == 0) mbar_arrive_cluster_relaxed(shared_bar);
       if (ok && row0 < args.M) {
         const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (acc ? 256u - C::kOver : 0u) +
                                static_cast<uint32_t>(half * kHalfCols);

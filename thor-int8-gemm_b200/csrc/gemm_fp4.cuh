@@ -469,7 +469,8 @@ __device__ __noinline__ void store_tail(const Args& args, const uint8_t* buf, in
 // `shared`: this half holds the columns that the other accumulator uses too, its last ones if half is
 // 1 and its first if it is 0; they are read first and `shared_bar` (the leader's, a cluster
 // address) is then told.
-template <bool MX, int OUT>
+// SCALED: the values are multiplied by row and weight scales.
+template <bool MX, int OUT, bool SCALED>
 __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMap* tm_out,
                                               typename PairCfg<MX, OUT>::Smem& s, int ew, int half,
                                               const GatedSlice& gs, uint32_t t_row, int row0, int n0, int lane,
@@ -513,7 +514,7 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
       const uint4* bq2 = reinterpret_cast<const uint4*>(tp.bias + (half * kHalfCols + c * kCols) / 2);
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        const float4 w0 = wq[2 * q], w1 = wq[2 * q + 1];
+        const float4 w0 = SCALED ? wq[2 * q] : float4{}, w1 = SCALED ? wq[2 * q + 1] : float4{};
         const float2 wp[4] = {make_float2(w0.x, w0.y), make_float2(w0.z, w0.w), make_float2(w1.x, w1.y),
                               make_float2(w1.z, w1.w)};
         const uint4 b4 = has_bias ? bq2[q] : make_uint4(0, 0, 0, 0);
@@ -531,7 +532,8 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
         uint32_t o[4];
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
-          float2 f = mul2_rn(mul2_rn(make_float2(v[8 * q + 2 * p], v[8 * q + 2 * p + 1]), xs2), wp[p]);
+          float2 f = make_float2(v[8 * q + 2 * p], v[8 * q + 2 * p + 1]);
+          if constexpr (SCALED) f = mul2_rn(mul2_rn(f, xs2), wp[p]);
           if (has_bias) f = add_f32_bf16x2(f, bw[p]);
           o[p] = f2_to_bf2(fma2_rn(bf2_to_f2(gw[p]), f, bf2_to_f2(rw[p])));
         }
@@ -544,17 +546,20 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
         if constexpr (OUT == kOutF32) {
-          const float4 w4 = wq[q];
           const uint4 b4 = bq[q];
-          float2 f0 = mul2_rn(mul2_rn(make_float2(v[4 * q], v[4 * q + 1]), xs2), make_float2(w4.x, w4.y));
-          float2 f1 = mul2_rn(mul2_rn(make_float2(v[4 * q + 2], v[4 * q + 3]), xs2), make_float2(w4.z, w4.w));
+          float2 f0 = make_float2(v[4 * q], v[4 * q + 1]), f1 = make_float2(v[4 * q + 2], v[4 * q + 3]);
+          if constexpr (SCALED) {
+            const float4 w4 = wq[q];
+            f0 = mul2_rn(mul2_rn(f0, xs2), make_float2(w4.x, w4.y));
+            f1 = mul2_rn(mul2_rn(f1, xs2), make_float2(w4.z, w4.w));
+          }
           if (has_bias) {
             f0 = make_float2(__fadd_rn(f0.x, __uint_as_float(b4.x)), __fadd_rn(f0.y, __uint_as_float(b4.y)));
             f1 = make_float2(__fadd_rn(f1.x, __uint_as_float(b4.z)), __fadd_rn(f1.y, __uint_as_float(b4.w)));
           }
           o[q] = make_uint4(__float_as_uint(f0.x), __float_as_uint(f0.y), __float_as_uint(f1.x), __float_as_uint(f1.y));
         } else {
-          const float4 w0 = wq[2 * q], w1 = wq[2 * q + 1];
+          const float4 w0 = SCALED ? wq[2 * q] : float4{}, w1 = SCALED ? wq[2 * q + 1] : float4{};
           const float2 wp[4] = {make_float2(w0.x, w0.y), make_float2(w0.z, w0.w), make_float2(w1.x, w1.y),
                                 make_float2(w1.z, w1.w)};
           const uint4 b4 = has_bias ? bq[q] : make_uint4(0, 0, 0, 0);
@@ -562,7 +567,8 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
           uint32_t h[4];
 #pragma unroll
           for (int p = 0; p < 4; ++p) {
-            float2 f = mul2_rn(mul2_rn(make_float2(v[8 * q + 2 * p], v[8 * q + 2 * p + 1]), xs2), wp[p]);
+            float2 f = make_float2(v[8 * q + 2 * p], v[8 * q + 2 * p + 1]);
+            if constexpr (SCALED) f = mul2_rn(mul2_rn(f, xs2), wp[p]);
             if (has_bias) f = OUT == kOutF16 ? add_f32_f16x2(f, bw[p]) : add_f32_bf16x2(f, bw[p]);
             h[p] = OutTraits<OUT>::pack2(f.x, f.y);
           }
@@ -588,7 +594,7 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
   }
 }
 
-template <bool MX, int OUT>
+template <bool MX, int OUT, bool SCALED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     gemm_fp4_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                          const __grid_constant__ CUtensorMap tm_sfa, const __grid_constant__ CUtensorMap tm_sfb,
@@ -774,8 +780,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       if (ok && row0 < args.M) {
         const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (acc ? 256u - C::kOver : 0u) +
                                static_cast<uint32_t>(half * kHalfCols);
-        epilogue_pair<MX, OUT>(args, &tm_out, s, ew, half, gs, t_row, row0, n0, lane, pol_out, xs_r, s.params[acc],
-                               shared, shared_bar);
+        epilogue_pair<MX, OUT, SCALED>(args, &tm_out, s, ew, half, gs, t_row, row0, n0, lane, pol_out, xs_r, s.params[acc],
+                                       shared, shared_bar);
       }
     }
     if constexpr (OUT == kOutGated) cp_async_wait_all();   // a residual copy left by a wait that gave up

@@ -191,6 +191,26 @@ def test_tiles_without_work_for_some_warps(kind, m, n, k):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", (520, 552, 576, 640, 648, 680, 744, 768))
+def test_gated_last_columns(kind, n):
+    """The gated form where the columns end in each 32 of a tile's row slice, in a padded residual updated in place:
+    the same values, and what lies past the columns and rows stays."""
+    m, k = 333, 264
+    g = gen(n)
+    x, w = ops.quant_rows_fp4(randn(g, m, k), kind), ops.quant_rows_fp4(randn(g, n, k, scale=0.02), kind)
+    big, gate = randn(g, m + 3, n + 8), randn(g, 5, n)
+    keep, res = big.clone(), big[:m, :n]
+    idx = torch.randint(0, 5, (m,), generator=g, device=DEV, dtype=torch.int32)
+    val = lambda o: ops.dequant_rows_fp4(*o, kind, out_dtype=torch.float32).double()  # noqa: E731
+    y = val(x) @ val(w).t()
+    want = res.double() + gate.double()[idx.long()] * y
+    ops.gemm_fp4_gated(x[0], w[0], x[1], w[1], x[2], w[2], None, res, gate, gate_index=idx, kind=kind, out=res)
+    # half a bf16 unit, and float32 accumulation far below 2^-14 of these operands' sums
+    assert ((res.double() - want).abs() <= want.abs() * 2.0 ** -8 + 2.0 ** -14 * (gate.abs().max() * y.abs().max())).all()
+    assert torch.equal(big[m:], keep[m:]) and torch.equal(big[:, n:], keep[:, n:])
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_scales_and_repeats(kind):
     """Row and weight scales in their forms (a row, one for all, none), an operand without a row scale,
     and the same bits from the same call, with K split over a cluster and not."""

@@ -477,7 +477,11 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
                                               const GatedSlice& gs, uint32_t t_row, int row0, int n0, int lane,
                                               uint64_t pol_out, float xs_r, const PairParams<OUT>& tp, bool shared,
                                               uint32_t shared_bar) {
-  constexpr int kCols = OUT == kOutF32 ? 32 : 64;
+  // 64 columns at a time; 32 for 4-byte outputs (a 128-byte piece of a row) and in mxfp4's gated form, whose
+  // accumulators share 32 columns and are told free that much earlier (16384 x 9216 x 3072: 198 us, 206 with 64;
+  // nvfp4 shares 64: 222, 216)
+  constexpr int kCols = (OUT == kOutF32 || (OUT == kOutGated && MX)) ? 32 : 64;
+  constexpr int kPieceChunks = OUT == kOutGated ? 64 / kCols : 1;
   constexpr int kChunks = kHalfCols / kCols;
   constexpr int kFirst = (PairCfg<MX, OUT>::kOver + kCols - 1) / kCols;   // chunks that hold the shared columns
   const bool has_bias = args.bias != nullptr;
@@ -510,22 +514,22 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
     if (i + 1 < kChunks) load(i + 1);
     if (c * kCols >= cols) continue;
     const float4* wq = reinterpret_cast<const float4*>(tp.ws + half * kHalfCols + c * kCols);
-    uint8_t* buf = s.epi[ew][OUT == kOutGated ? c : 0];
+    uint8_t* buf = s.epi[ew][OUT == kOutGated ? c / kPieceChunks : 0];
     if constexpr (OUT == kOutGated) {
       const uint4* bq2 = reinterpret_cast<const uint4*>(tp.bias + (half * kHalfCols + c * kCols) / 2);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
+      for (int q = 0; q < kCols / 8; ++q) {
         const float4 w0 = SCALED ? wq[2 * q] : float4{}, w1 = SCALED ? wq[2 * q + 1] : float4{};
         const float2 wp[4] = {make_float2(w0.x, w0.y), make_float2(w0.z, w0.w), make_float2(w1.x, w1.y),
                               make_float2(w1.z, w1.w)};
         const uint4 b4 = has_bias ? bq2[q] : make_uint4(0, 0, 0, 0);
         const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w};
         const int col = c * kCols + 8 * q;
-        uint4* cell = reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) * 16));
+        uint4* cell = reinterpret_cast<uint4*>(buf + lane * 128 + (((q + c % kPieceChunks * 4) ^ (lane & 7)) * 16));
         const uint4 r4 = *cell;
         uint4 g4 = make_uint4(0, 0, 0, 0);
         if (gs.shared_gate)
-          g4 = *reinterpret_cast<const uint4*>(s.gate[ew] + (c * 8 + q) * 16);
+          g4 = *reinterpret_cast<const uint4*>(s.gate[ew] + (c * (kCols / 8) + q) * 16);
         else if (gs.gate_row != nullptr && col < cols)
           g4 = __ldg(reinterpret_cast<const uint4*>(gs.gate_row + col));
         const uint32_t rw[4] = {r4.x, r4.y, r4.z, r4.w};
@@ -586,10 +590,15 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
       const int left = cols - c * kCols;
       if (left < kCols && left % kPer != 0 && row0 + lane < args.M) store_tail<OUT>(args, buf, lane, row0, n0 + c * kCols, left);
     }
+    if constexpr (kPieceChunks == 2) {
+      // a piece is stored with its second chunk, or with its only one before N (the skipped one is the upper,
+      // which the other half's order takes first)
+      if (i % 2 == 0 && (half == 1 || (c + 1) * kCols < cols)) continue;
+    }
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-      tma_store_2d(tm_out, buf, n0 + c * kCols, row0, pol_out);
+      tma_store_2d(tm_out, buf, n0 + c / kPieceChunks * (kPieceChunks * kCols), row0, pol_out);
       bulk_commit_group();
     }
   }

@@ -487,10 +487,6 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
   const bool has_bias = args.bias != nullptr;
   const float2 xs2 = make_float2(xs_r, xs_r);
   const int cols = args.N - n0;
-  if constexpr (OUT == kOutGated) {
-    cp_async_wait_all();
-    __syncwarp();
-  }
   uint32_t r[kCols / 32][32];
   auto load = [&](int i) {
     const int c = half ? kChunks - 1 - i : i;
@@ -512,6 +508,12 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
       if (lane == 0) mbar_arrive_cluster_relaxed(shared_bar);
     }
     if (i + 1 < kChunks) load(i + 1);
+    if constexpr (OUT == kOutGated) {
+      if (i == 0) {   // the residual is in (the next tile's MMAs do not wait for it)
+        cp_async_wait_all();
+        __syncwarp();
+      }
+    }
     if (c * kCols >= cols) continue;
     const float4* wq = reinterpret_cast<const float4*>(tp.ws + half * kHalfCols + c * kCols);
     uint8_t* buf = s.epi[ew][OUT == kOutGated ? c / kPieceChunks : 0];

@@ -1,0 +1,68 @@
+"""Forms of the 4-bit operators in which tiles, scales and special values meet, and repeated calls."""
+import pytest
+import torch
+
+from test_gpu_fp4 import check_operand
+from thor_int8_gemm_b200 import ops
+
+pytestmark = pytest.mark.gpu
+KINDS = ("mxfp4", "nvfp4")
+DEV = "cuda:0"
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    assert ops.device_status() == 0
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def randn(g, *s, scale=1.0):
+    return (torch.randn(*s, generator=g, device=DEV) * scale).to(torch.bfloat16)
+
+
+# ---------------------------------------------------------------- the same inputs, and the definition in 64 bits
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("op,m,n,k", [("swiglu", 77, 640, 2568), ("swiglu", 420, 64, 1552), ("norm", 300, 520, 1288),
+                                      ("norm", 2100, 264, 1024), ("quant", 130, 200, 776)])
+def test_repeats_whatever_ran_between(kind, op, m, n, k):
+    """A quantiser and the product behind it give the same bits for the same inputs, whatever other inputs, and
+    whatever freed memory their outputs land in, came between."""
+    g = gen(m + k)
+    w = ops.quant_rows_fp4(randn(g, n, k, scale=0.02), kind)
+    shift, scale, res, gate = randn(g, 1, k, scale=0.1), randn(g, 1, k, scale=0.1), randn(g, m, n), randn(g, 1, n)
+    inputs = [randn(g, m, 2 * k if op == "swiglu" else k) for _ in range(2)]
+
+    def run(x):
+        if op == "swiglu":
+            a = ops.swiglu_quant_fp4_fc1(x, kind)
+        elif op == "norm":
+            a = ops.rms_mod_quant_fp4(x, shift, scale, rows_per_mod=m, kind=kind)
+        else:
+            a = ops.quant_rows_fp4(x, kind)
+        return ops.gemm_fp4_gated(a[0], w[0], a[1], w[1], a[2], w[2], None, res, gate, rows_per_gate=m, kind=kind)
+
+    first = [run(x) for x in inputs]
+    for turn in range(12):
+        soiled = [torch.full((size,), 37 * turn % 256, dtype=torch.uint8, device=DEV) for size in (512, 4096, 40000, 400000)]
+        del soiled
+        for x, want in zip(inputs, first):
+            assert torch.equal(run(x), want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_swiglu_codes_against_64_bits(kind):
+    """The codes are those of act, and act is the float64 value rounded to bf16 but for what its float32
+    evaluation adds: five roundings (exp, 1 + e, the division, g * s, the product with up) of 2^-24 each, below 2^-21, beside
+    half a bf16 unit.  So a code that differs from the float64 value's belongs to an act that near the border between two
+    bf16 values."""
+    y = randn(gen(13), 300, 2 * 2568)
+    act = ops.swiglu_quant_fc1(y, "int8", return_act=True)[2]
+    check_operand(ops.swiglu_quant_fp4_fc1(y, kind), act.cpu(), kind)
+    g, u = y.double().chunk(2, 1)
+    exact = g / (1 + torch.exp(-g)) * u
+    half_unit = torch.exp2(torch.floor(torch.log2(exact.abs().clamp(min=2.0 ** -126))) - 8)
+    assert ((act.double() - exact).abs() <= half_unit + exact.abs() * 2.0 ** -21).all()

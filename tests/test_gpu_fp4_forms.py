@@ -66,3 +66,46 @@ def test_swiglu_codes_against_64_bits(kind):
     exact = g / (1 + torch.exp(-g)) * u
     half_unit = torch.exp2(torch.floor(torch.log2(exact.abs().clamp(min=2.0 ** -126))) - 8)
     assert ((act.double() - exact).abs() <= half_unit + exact.abs() * 2.0 ** -21).all()
+
+
+def value(op, kind):
+    return ops.dequant_rows_fp4(*op, kind, out_dtype=torch.float32).double()
+
+
+# ---------------------------------------------------------------- products of many tiles
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,n,k,form", [(4921, 4112, 520, "rows"), (2305, 9229, 264, "one"), (4921, 4112, 8, "none")])
+def test_many_tiles_in_every_output_type(kind, dtype, m, n, k, form):
+    """340 and 370 output tiles over at most 74 CTA pairs: both accumulators and the columns that they share, a tile's first
+    scales copied early (K of more than 256) and not, with row and weight scales, one weight scale, and the operands' own.
+
+    Tolerance: K / 64 accumulation steps as in test_gpu_fp4.tolerance (a unit of the sum of magnitudes for each addition and
+    each K = 64 sum), three float32 roundings of the scaled sum and of the sum with the bias (2^-24 each, below
+    2^-22 of the larger), half a unit of the output type (half its smallest number where it is subnormal)."""
+    g = gen(m + n + k)
+    x, w = ops.quant_rows_fp4(randn(g, m, k), kind), ops.quant_rows_fp4(randn(g, n, k, scale=0.02), kind)
+    xs, ws = x[2], w[2]
+    xv, wv = value((x[0], x[1], None), kind), value((w[0], w[1], None), kind)
+    if form != "none":
+        xs = (torch.rand(m, generator=g, device=DEV) + 0.5) * (1 if xs is None else xs)
+        ws = torch.rand(n if form == "rows" else 1, generator=g, device=DEV) + 0.5
+        if w[2] is not None:   # nvfp4: near the scales that the weight was quantised with
+            ws = ws * (w[2] if form == "rows" else w[2].median())
+    bias = randn(g, n, scale=0.1).to(dtype)
+    scale = 1.0
+    if xs is not None:
+        scale = scale * xs.double()[:, None]
+    if ws is not None:
+        scale = scale * ws.double()
+    y = xv @ wv.t() * scale
+    want = y + bias.double()
+    fi = torch.finfo(dtype)
+    tol = (xv.abs() @ wv.abs().t() * scale) * (2.0 ** -23 * (2 * -(-k // 64) + 2)) + torch.maximum(y.abs(), want.abs()) * 2.0 ** -22
+    tol += want.abs() * (fi.eps / 2) + fi.tiny * fi.eps / 2
+    first = None
+    for _ in range(4):
+        out = ops.gemm_fp4(x[0], w[0], x[1], w[1], xs, ws, bias, kind=kind, out_dtype=dtype)
+        assert ((out.double() - want).abs() <= tol).all()
+        first = out if first is None else first
+        assert torch.equal(out, first)

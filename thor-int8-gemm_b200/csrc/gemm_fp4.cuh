@@ -466,6 +466,14 @@ __device__ __noinline__ void store_tail(const Args& args, const uint8_t* buf, in
   }
 }
 
+// A warp's report that its reads of TMEM so far are done: what the MMAs behind `bar` (a cluster address) may
+// overwrite.  Every lane's loads are complete (tcgen05.wait::ld) and ordered before the arrival by its own fence.
+__device__ __forceinline__ void report_read(uint32_t bar, int lane) {
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive_cluster_relaxed(bar);
+}
+
 // Epilogue of a warp's 32 x 128 slice of a tile (columns n0 .. of the output, `half` of the tile).
 // `shared`: this half holds the columns that the other accumulator uses too, its last ones if half is
 // 1 and its first if it is 0; they are read first and `shared_bar` (the leader's, a cluster
@@ -502,11 +510,7 @@ __device__ __forceinline__ void epilogue_pair(const Args& args, const CUtensorMa
     float v[kCols];
 #pragma unroll
     for (int j = 0; j < kCols; ++j) v[j] = __uint_as_float(r[j / 32][j % 32]);
-    if (shared && i == kFirst - 1) {   // the next tile's MMAs wait for this
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster_relaxed(shared_bar);
-    }
+    if (shared && i == kFirst - 1) report_read(shared_bar, lane);   // the next tile's MMAs wait for this
     if (i + 1 < kChunks) load(i + 1);
     if constexpr (OUT == kOutGated) {
       if (i == 0) {   // the residual is in (the next tile's MMAs do not wait for it)
@@ -788,7 +792,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       // The other half, and a warp without rows, report as well, which tells that they are done with the tile
       // before.  Only now: this tile's MMAs began when the tile before had all its reports, so no warp's
       // report for this tile can be taken for a slower warp's for that one.
-      if (ok && !shared && lane == 0) mbar_arrive_cluster_relaxed(shared_bar);
+      if (ok && !shared) report_read(shared_bar, lane);
       if (ok && row0 < args.M) {
         const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + (acc ? 256u - C::kOver : 0u) +
                                static_cast<uint32_t>(half * kHalfCols);

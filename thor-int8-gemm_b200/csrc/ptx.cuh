@@ -511,9 +511,10 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
   return __all_sync(0xFFFFFFFFu, mbar_wait_sleep(bar, parity, code));
 }
 
-// Arrive anywhere in the cluster without ordering this thread's memory accesses: enough to hand TMEM
-// columns over (their loads are complete and a tcgen05 fence precedes it), and it does not wait
-// for the thread's outstanding stores as a cluster-scope release does.
+// Arrive anywhere in the cluster without ordering this thread's memory accesses.  For handing TMEM columns over,
+// between tcgen05.wait::ld + tcgen05.fence::before_thread_sync on this side and tcgen05.fence::after_thread_sync
+// behind the wait on the other: those fences order the tensor-memory accesses, the arrival only has to be
+// seen.  A cluster-scope release would wait for the thread's outstanding stores as well.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }

@@ -286,7 +286,8 @@ int64_t t8g_fp4_scale_bytes(int64_t rows, int64_t K, int quant_kind);
  * nvfp4 block scale = e4m3(amax / (6 * 2^r)); code = e2m1(x / scale), to nearest, ties to even,
  * saturating at 6.  A block (mxfp4) or row (nvfp4) that holds a NaN or an infinity gets a NaN scale.
  *   x [S, D] bf16 (ld_x), q and sf as above, q_scale [S] float32 (NULL for mxfp4).
- * The scales of rows S .. next multiple of 128 are left as they were.
+ * The scales of rows S .. next multiple of 128 are left as they were.  S == 0 is a no-op; of rows without elements
+ * (D == 0) only nvfp4's row scales are written, as of rows of zeros (2^-100), if q_scale is given.
  * Requirements: D a multiple of 8, D <= 49152; x 16-byte aligned, ld_x a multiple of 8.
  */
 int t8g_quant_rows_fp4(const void* x, int64_t ld_x, void* q, int64_t ld_q, void* sf, float* q_scale, int64_t S,

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from test_gpu_fp4 import check_operand
-from thor_int8_gemm_b200 import ops
+from thor_int8_gemm_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 KINDS = ("mxfp4", "nvfp4")
@@ -109,3 +109,23 @@ def test_many_tiles_in_every_output_type(kind, dtype, m, n, k, form):
         assert ((out.double() - want).abs() <= tol).all()
         first = out if first is None else first
         assert torch.equal(out, first)
+
+
+# ---------------------------------------------------------------- rows without elements
+def test_rows_without_elements_have_the_scale_of_zeros():
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    for call in (lambda s: lib.t8g_quant_rows_fp4(None, 0, None, 0, None, s, 300, 0, _lib.QUANT_NVFP4, stream),
+                 lambda s: lib.t8g_rms_mod_quant_fp4(None, 0, None, None, None, 0, None, 300, 0, 1e-6, None, 0, None, s, 300, 0,
+                                                     _lib.QUANT_NVFP4, stream),
+                 lambda s: lib.t8g_swiglu_quant_fp4(None, None, 0, None, 0, None, s, 300, 0, _lib.QUANT_NVFP4, stream)):
+        scale = torch.full((301,), 7.0, device=DEV)
+        assert call(scale.data_ptr()) == 0
+        assert (scale[:300] == 2.0 ** -100).all() and scale[300] == 7
+    e = torch.empty(5, 0, dtype=torch.bfloat16, device=DEV)
+    zeros = ops.quant_rows_fp4(torch.zeros(5, 16, dtype=torch.bfloat16, device=DEV), "nvfp4")[2]
+    m = torch.empty(1, 0, dtype=torch.bfloat16, device=DEV)
+    for q, sf, s in (ops.quant_rows_fp4(e, "nvfp4"), ops.swiglu_quant_fp4_fc1(e, "nvfp4"), ops.swiglu_quant_fp4(e, e, "nvfp4"),
+                     ops.rms_mod_quant_fp4(e, m, m, rows_per_mod=5, kind="nvfp4")):
+        assert q.shape == (5, 0) and sf.numel() == 0 and torch.equal(s, zeros)
+        assert ops.dequant_rows_fp4(q, sf, s, "nvfp4").shape == (5, 0)
+    assert ops.quant_rows_fp4(e, "mxfp4")[2] is None

@@ -71,6 +71,15 @@ __device__ __forceinline__ float row_scale_fp4(uint32_t amax, float* inverse) {
   return __uint_as_float(static_cast<uint32_t>(127 + r) << 23);
 }
 
+// The row scales of S rows of zeros.
+__global__ void __launch_bounds__(256) zero_row_scales_fp4_kernel(float* q_scale, int64_t S) {
+  float inverse;
+  const float scale = row_scale_fp4(0u, &inverse);
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; row < S;
+       row += static_cast<int64_t>(gridDim.x) * blockDim.x)
+    q_scale[row] = scale;
+}
+
 // Eight fp32 values -> eight e2m1 codes (first value in the lowest four bits).
 __device__ __forceinline__ uint32_t cvt_e2m1x8(const float2 (&v)[4]) {
   uint32_t r;

@@ -43,6 +43,19 @@ t8g::rows::Fp4Out fp4_out(void* q, int64_t ld_q, void* sf, float* q_scale, int64
   return o;
 }
 
+// Rows without elements: no codes and no block scales, but nvfp4's row scales, which are those of rows of zeros.
+int empty_rows_fp4(const char* what, float* q_scale, int64_t S, int kind, void* stream) {
+  if (kind != T8G_QUANT_NVFP4 || !q_scale) return T8G_OK;
+  if (!aligned(q_scale, 4)) return fail(T8G_ERR_INVALID_ARGUMENT, "%s: row scales must be 4-byte aligned", what);
+  int dev;
+  DeviceInfo info;
+  const int rc = current_device(&dev, &info);
+  if (rc) return rc;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((S + 255) / 256, 8 * info.sms));
+  t8g::rows::zero_row_scales_fp4_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(q_scale, S);
+  return launch_checked(what);
+}
+
 // Vectors per thread of a direct row kernel: the canonical shape's, rounded up to a compiled one.
 #define T8G_DISPATCH_FP4_V(v, ...)                     \
   if ((v) <= 3) {                                      \
@@ -304,7 +317,8 @@ int t8g_quant_rows_fp4(const void* x, int64_t ld_x, void* q, int64_t ld_q, void*
                        int quant_kind, void* stream) {
   using namespace t8g::rows;
   int rc = check_fp4_rows("quant_rows_fp4", S, D, quant_kind, 49152);
-  if (rc || S == 0 || D == 0) return rc;
+  if (rc || S == 0) return rc;
+  if (D == 0) return empty_rows_fp4("quant_rows_fp4", q_scale, S, quant_kind, stream);
   if ((rc = check_bf16_matrix("x", x, ld_x, D, true))) return rc;
   if ((rc = check_fp4_operand("q", q, ld_q, sf, q_scale, D, quant_kind, true))) return rc;
   int dev;
@@ -326,7 +340,8 @@ int t8g_rms_mod_quant_fp4(const void* x, int64_t ld_x, const void* w, const void
                           int quant_kind, void* stream) {
   using namespace t8g::rows;
   int rc = check_fp4_rows("rms_mod_quant_fp4", S, D, quant_kind, 49152);
-  if (rc || S == 0 || D == 0) return rc;
+  if (rc || S == 0) return rc;
+  if (D == 0) return empty_rows_fp4("rms_mod_quant_fp4", q_scale, S, quant_kind, stream);
   if ((rc = check_bf16_matrix("x", x, ld_x, D, true))) return rc;
   if ((rc = check_bf16_matrix("shift", shift, ld_mod, D, true))) return rc;
   if ((rc = check_bf16_matrix("scale", scale, ld_mod, D, true))) return rc;
@@ -360,7 +375,8 @@ int t8g_swiglu_quant_fp4(const void* gate, const void* up, int64_t ld_in, void* 
                          int64_t M, int64_t F, int quant_kind, void* stream) {
   using namespace t8g::rows;
   int rc = check_fp4_rows("swiglu_quant_fp4", M, F, quant_kind, 24576);
-  if (rc || M == 0 || F == 0) return rc;
+  if (rc || M == 0) return rc;
+  if (F == 0) return empty_rows_fp4("swiglu_quant_fp4", q_scale, M, quant_kind, stream);
   if ((rc = check_bf16_matrix("gate", gate, ld_in, F, true))) return rc;
   if ((rc = check_bf16_matrix("up", up, ld_in, F, true))) return rc;
   if ((rc = check_fp4_operand("q", q, ld_q, sf, q_scale, F, quant_kind, true))) return rc;

@@ -1,5 +1,6 @@
 """Microscaled 4-bit operators, what needs no GPU: the oracle, the layout, refusals, custom-op shapes."""
 import ctypes
+import sys
 
 import numpy as np
 import pytest
@@ -182,6 +183,22 @@ def test_compiled_call_path_declines():
     for f in (F.gemm, F.gated, F.dequant, F.quant_rows, F.swiglu_fc1, F.rms_mod_quant, F.setup):
         with pytest.raises(TypeError):
             f(q)
+
+
+def test_missing_call_path_leaves_the_general_one(monkeypatch):
+    """Without the compiled call path (not built, or for another Python) the wrappers go on to the general path, which
+    refuses host tensors here and launches on a GPU."""
+    name = f"{ops.__package__}._t8g_fp4"
+    monkeypatch.setattr(ops, "_fp4_module", None)
+    monkeypatch.delattr(sys.modules[ops.__package__], "_t8g_fp4", raising=False)
+    monkeypatch.setitem(sys.modules, name, None)   # the import statement raises ImportError
+    x, q, sf = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8)
+    for call in (lambda: ops.quant_rows_fp4(x, "mxfp4"), lambda: ops.swiglu_quant_fp4_fc1(x, "nvfp4"),
+                 lambda: ops.rms_mod_quant_fp4(x, x[:1], x[:1], rows_per_mod=4),
+                 lambda: ops.dequant_rows_fp4(q, sf, None, "mxfp4"), lambda: ops.gemm_fp4(q, q, sf, sf, kind="mxfp4"),
+                 lambda: ops.gemm_fp4_gated(q, q, sf, sf, None, None, None, x[:, :4], x[:1, :4], rows_per_gate=4)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
 
 
 @pytest.mark.parametrize("kind", KINDS)

@@ -496,6 +496,17 @@ FP4_CODE = {"mxfp4": _lib.QUANT_MXFP4, "nvfp4": _lib.QUANT_NVFP4}
 FP4_BLOCK = {"mxfp4": 32, "nvfp4": 16}
 
 
+class _NoCallPath:
+    """In the compiled call path's place where that module is not built (or for another Python): every call
+    takes the general path."""
+
+    @staticmethod
+    def _declines(*args) -> bool:
+        return False
+
+    gemm = gated = quant_rows = swiglu_fc1 = rms_mod_quant = dequant = _declines
+
+
 _fp4_module = None
 
 
@@ -504,8 +515,12 @@ def _fp4_fast():
     when it launched, False for the general path below, or the library's status."""
     global _fp4_module
     if _fp4_module is None:
-        _lib.load()
-        from . import _t8g_fp4
+        _lib.load()   # raises where the library itself is missing
+        try:
+            from . import _t8g_fp4
+        except ImportError:
+            _fp4_module = _NoCallPath
+            return _fp4_module
         raw = _raw_stream or (lambda idx: torch.cuda.current_stream(idx).cuda_stream)
         _t8g_fp4.setup(torch.uint8, torch.float32, torch.bfloat16, raw)
         _fp4_module = _t8g_fp4

@@ -113,8 +113,10 @@ int encode_2d_uncached(CUtensorMap* m, CUtensorMapDataType dt, const void* base,
   return T8G_OK;
 }
 
-// Recently encoded tensor maps of this thread: a layer calls the GEMM with the same weight,
-// and often the same activation and output buffers, every step, so most maps repeat.
+// Recently encoded tensor maps of this thread.  A call that is repeated finds all of its maps (three, 4-bit
+// products four or five); a loop over the linears of a block finds those of shared buffers at most, its weights'
+// are encoded anew.  That is cheap: two maps anew in every 4-bit product (8 or 200 weights in turn) cost
+// 0.3 us of its 6 us on the host, and 1024 hashed entries in place of these 16 took off no more than that.
 struct MapKey {
   const void* base;
   uint64_t inner, outer, ld_bytes;

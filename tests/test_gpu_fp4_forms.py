@@ -1,4 +1,4 @@
-"""Forms of the 4-bit operators in which tiles, scales and special values meet, and repeated calls."""
+"""Forms of the 4-bit operators in which tiles, scales and special values meet, bytes that are not theirs, and repeated calls."""
 import pytest
 import torch
 
@@ -129,3 +129,106 @@ def test_rows_without_elements_have_the_scale_of_zeros():
         assert q.shape == (5, 0) and sf.numel() == 0 and torch.equal(s, zeros)
         assert ops.dequant_rows_fp4(q, sf, s, "nvfp4").shape == (5, 0)
     assert ops.quant_rows_fp4(e, "mxfp4")[2] is None
+
+
+# ---------------------------------------------------------------- special values behind a norm and a SwiGLU
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("s,d", [(60, 1536), (2060, 1536), (2100, 1024), (2052, 4096), (33, 264), (7, 8200)])
+def test_norm_of_special_values(kind, s, d):
+    """NaN and infinities in x and in the modulation, and h that is finite in float32 but past bf16's largest number (3.3895e38
+    times a normalised 1, plus 1e36), in rows of the register kernel (2048 rows and more of 256 n) and of the others:
+    the same operand as quantising the stored h."""
+    g = gen(d + s)
+    x, shift, scale = randn(g, s, d), randn(g, 4, d), randn(g, 4, d)
+    idx = torch.randint(0, 2, (s,), generator=g, device=DEV, dtype=torch.int32)
+    top = torch.finfo(torch.bfloat16).max
+    x[1, 3], x[2, d - 1], x[s - 1, d // 2] = float("nan"), float("inf"), -float("inf")
+    x[3] = 0
+    x[4] = 1.0
+    scale[2], shift[2] = top, 1e36
+    idx[4] = 2
+    scale[3, 5], shift[3, d - 9] = float("inf"), float("nan")
+    idx[5] = idx[s - 2] = 3
+    x[6] = torch.randn(d, generator=g, device=DEV).bfloat16() * 1e-38   # subnormal h under a multiplier of 1e-3
+    kw = dict(mod_index=idx, scale_is_multiplier=True, eps=1e-6)
+    h = ops.rms_mod_quant(x, shift, scale, kind="int8", return_h=True, **kw)[2]
+    assert h[4].isinf().all() and h[[1, 2]].isnan().any(1).all()
+    check_operand(ops.rms_mod_quant_fp4(x, shift, scale, kind=kind, **kw), h.cpu(), kind)
+    w = randn(g, d)
+    w[d - 2] = float("nan")
+    kw["w"] = w
+    h = ops.rms_mod_quant(x, shift, scale, kind="int8", return_h=True, **kw)[2]
+    check_operand(ops.rms_mod_quant_fp4(x, shift, scale, kind=kind, **kw), h.cpu(), kind)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,f", [(40, 136), (77, 2568), (900, 1536), (9, 24576)])
+def test_swiglu_of_special_values(kind, m, f):
+    """NaN and infinities in gate and up (-inf * 0 is NaN), act past bf16's largest number and act among its
+    subnormals: the same operand as quantising the stored act."""
+    y = randn(gen(m + f), m, 2 * f)
+    y[1, 2], y[2, f + 1] = float("nan"), float("nan")
+    y[3, f - 1], y[4, 0] = float("inf"), -float("inf")
+    y[5, 2 * f - 1], y[m - 1, f + 5] = float("inf"), -float("inf")
+    y[6, 7], y[6, f + 7] = 3e38, 3e38
+    y[7, :f] = -88.0
+    y[8, f:] = y[8, f:] * 1e-38
+    act = ops.swiglu_quant_fc1(y, "int8", return_act=True)[2]
+    check_operand(ops.swiglu_quant_fp4_fc1(y, kind), act.cpu(), kind)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("s,form", [(2048, "batch"), (2304, "index"), (2049, "w")])
+def test_norm_of_many_rows_of_1536(kind, s, form):
+    g = gen(s)
+    d, n_mod = 1536, 3 if s % 3 == 0 else 1
+    x, shift, scale = randn(g, s, d), randn(g, n_mod, d), randn(g, n_mod, d)
+    kw = {}
+    if form == "index":
+        kw["mod_index"] = torch.randint(0, n_mod, (s,), generator=g, device=DEV, dtype=torch.int32)
+    if form == "w":
+        kw["w"] = randn(g, d)
+    h = ops.rms_mod_quant(x, shift, scale, kind="int8", return_h=True, **kw)[2]
+    check_operand(ops.rms_mod_quant_fp4(x, shift, scale, kind=kind, **kw), h.cpu(), kind)
+
+
+# ---------------------------------------------------------------- bytes that are not the call's
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("op,s,d", [("quant", 9, 136), ("quant", 129, 264), ("quant", 2500, 1024), ("norm", 35, 1288),
+                                    ("norm", 2049, 1024), ("norm", 2100, 1536), ("swiglu", 77, 2568), ("swiglu", 161, 40)])
+def test_other_bytes_stay(kind, op, s, d):
+    """Through the C entry, into buffers that hold something: the bytes between a row's codes and the next row, the block scales
+    of rows past the last (up to a multiple of 128) and what lies behind the buffers are left; the rest is the call's,
+    whatever the pitch."""
+    g = gen(s + d)
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    code = ops.FP4_CODE[kind]
+    pitch, n_sf = -(-d // 32) * 16 + 48, ops.fp4_scale_bytes(s, d, kind)
+    q = torch.full((s + 1, pitch), 0xA5, dtype=torch.uint8, device=DEV)
+    sf = torch.full((n_sf + 512,), 0xA5, dtype=torch.uint8, device=DEV)
+    qs = torch.full((s + 1,), 7.0, device=DEV)
+    scale = qs.data_ptr() if kind == "nvfp4" else None
+    to = (q.data_ptr(), pitch, sf.data_ptr(), scale, s, d, code, stream)
+    big = randn(g, s, 2 * d + 24)
+    if op == "quant":
+        rc = lib.t8g_quant_rows_fp4(big.data_ptr(), big.stride(0), *to)
+        want = ops.quant_rows_fp4(big[:, :d], kind)
+    elif op == "norm":
+        mod = randn(g, 2, d + 8)
+        rc = lib.t8g_rms_mod_quant_fp4(big.data_ptr(), big.stride(0), None, mod[0].data_ptr(), mod[1].data_ptr(), d + 8, None, s, 0,
+                                       1e-6, *to)
+        want = ops.rms_mod_quant_fp4(big[:, :d], mod[:1, :d], mod[1:, :d], rows_per_mod=s, eps=1e-6, kind=kind)
+    else:
+        rc = lib.t8g_swiglu_quant_fp4(big.data_ptr(), big.data_ptr() + 2 * (d + 8), big.stride(0), *to)
+        want = ops.swiglu_quant_fp4(big[:, :d], big[:, d + 8:2 * d + 8], kind)
+    assert rc == 0, lib.t8g_last_error()
+    assert torch.equal(q[:s, :d // 2], want[0])
+    assert (q[:s, d // 2:] == 0xA5).all() and (q[s] == 0xA5).all() and (sf[n_sf:] == 0xA5).all()
+    rows = sf[:n_sf].view(-(-s // 128), -1, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(-(-s // 128) * 128, -1)
+    assert (rows[s:] == 0xA5).all()
+    blocks = -(-d // ops.FP4_BLOCK[kind])
+    assert torch.equal(rows[:s, :blocks], ops.fp4_scale_rows(want[1], s, d, kind)) and (rows[:s, blocks:] == 0).all()
+    if kind == "nvfp4":
+        assert torch.equal(qs[:s], want[2]) and qs[s] == 7
+    else:
+        assert (qs == 7).all()

@@ -232,3 +232,15 @@ def test_other_bytes_stay(kind, op, s, d):
         assert torch.equal(qs[:s], want[2]) and qs[s] == 7
     else:
         assert (qs == 7).all()
+
+
+# ---------------------------------------------------------------- refusals
+def test_no_modulation_row_is_refused():
+    x, none = torch.ones(4, 64, dtype=torch.bfloat16, device=DEV), torch.empty(0, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="split evenly over 0"):
+        ops.rms_mod_quant_fp4(x, none, none)
+    with pytest.raises(ValueError, match="past the 0"):
+        ops.rms_mod_quant_fp4(x, none, none, rows_per_mod=4)
+    with pytest.raises(_lib.T8GError, match="shift is null"):
+        ops.rms_mod_quant_fp4(x, none, none, mod_index=torch.zeros(4, dtype=torch.int32, device=DEV))
+    assert ops.rms_mod_quant_fp4(none, none, none)[0].shape == (0, 32)

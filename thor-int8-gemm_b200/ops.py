@@ -379,9 +379,9 @@ def _mod_args(x, shift, scale, mod_index, rows_per_mod):
         rows_per_mod = 1
     elif rows_per_mod is None:
         n_mod = shift2.shape[0]
-        if S % n_mod:
+        if S and (not n_mod or S % n_mod):
             raise ValueError(f"{S} rows do not split evenly over {n_mod} modulation rows; pass mod_index")
-        rows_per_mod = max(S // n_mod, 1)
+        rows_per_mod = max(S // max(n_mod, 1), 1)
     return shift2, scale2, rows_per_mod
 
 

@@ -268,7 +268,8 @@ int t8g_rms_mod_quant_tensorwise_noalloc(const void* x, int64_t ld_x, const void
  *   sf       block scales in tiles of 128 rows x 4 blocks (512 bytes; row r, block b of a tile at byte
  *            (r % 32) * 16 + (r / 32) * 4 + b), a row group's tiles consecutive along K;
  *            t8g_fp4_scale_bytes(rows, K, kind) bytes, 16-byte aligned.  A caller that fills it
- *            itself sets the scales of blocks past the row's last one (up to a multiple of 4) to 0.
+ *            itself sets the scales of blocks past the row's last one (up to a multiple of 4) to 0; an
+ *            e4m3 scale's sign bit is 0.
  *   scale    float32 [rows] (weights: numel 1 or rows), or NULL for 1
  * and a value is code * block scale * row scale.
  *   T8G_QUANT_MXFP4  blocks of 32, e8m0 scales (the quantisers write no row scale)

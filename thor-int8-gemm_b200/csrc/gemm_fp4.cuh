@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 2)
 //     [0, 256)   [256 - kOver, 512 - kOver)   scales [512 - kOver, 512)
 // and a tile's epilogue reads the shared columns first and then reports them free, so that the next tile's
 // MMAs wait for one chunk of the epilogue, not for all of it.  (Tiles of 192 columns would need no
-// overlap, but feed the tensor cores 14 % more operand bytes per product.)
+// overlap, but feed the tensor cores 17 % more operand bytes per product.)
 // A CTA needs its own 128 rows' scales of A but those of all 256 rows of W: both CTAs load them.
 //
 // Eight epilogue warps share a CTA's half of a tile: warp 2 + 4 h + i reads the 32 lanes 32 ((2 + i) % 4) .. of columns [128 h, 128 h + 128).

@@ -8,11 +8,13 @@
 //   nvfp4: block of 16, row scale 2^r with the least r >= -100 that has amax(row) <= 6 * 448 * 2^r,
 //          block scale e4m3(amax / (6 * 2^r)).
 // The values quantised are bf16 (8 significant bits), also behind a norm or a SwiGLU, so that the
-// fused forms give exactly what quantising their stored bf16 result gives.  Every decision is
+// fused forms give exactly what quantising their stored bf16 result gives (where that lies next to a border between
+// two bf16 values, its float32 evaluation may round the other way than float64 would, and one code with it).  Every decision is
 // then exact in fp32: mxfp4's x / scale is a shift; for nvfp4 x / scale either is one of the seven
 // borders between e2m1 values or at least 2^-10 away from it (x and border * scale are both
 // integers of at most 8 bits on a common grid), so a quotient rounded to a multiple of 2^-14, which the fp32 adder does
-// (add and subtract 1.5 * 2^9), falls on the border exactly when x does.
+// (add and subtract 1.5 * 2^9), falls on the border exactly when x does (a negative x below 2^-15 of its scale becomes
+// the code of +0, where -0 would be its rounding).
 // A block with a NaN or an infinity has a NaN scale; a row with one has (nvfp4) a NaN row scale,
 // so every product with that row is NaN.
 //
@@ -253,7 +255,9 @@ enum Fp4Source : int { kFp4Plain = 0, kFp4Norm = 1, kFp4NormWeight = 2 };
 
 // rows_per_group rows for each group; a holds x (and, for the norm, its operands).
 // Three vectors a thread keep to 64 registers, so that two of the widest CTAs share an SM: with the next row
-// and the modulation held in registers the norm had one, and 8192 x 8192 mxfp4 took 96 us (now 81).
+// and the modulation held in registers the norm had one, and 8192 x 8192 mxfp4 took 96 us (now 74, nvfp4 87).  What is
+// left of the norm's distance from HBM (26 us) is that a row is loaded only when the one before is done, and that its
+// modulation is read again for every row.
 template <bool MX, int V, int SRC>
 __global__ void __launch_bounds__(512, V == 3 ? 2 : 1) rows_fp4_kernel(const RmsArgs a, const Fp4Out o, const int T,
                                                        const int64_t rows_per_group) {
@@ -328,8 +332,8 @@ __global__ void __launch_bounds__(512, V == 3 ? 2 : 1) rows_fp4_kernel(const Rms
 // vectors 32 k + l), so that the per-row work (sums, reciprocal square root, scale) is shared by NV
 // vectors a lane instead of three, and no warp waits for another; the modulation of the CTA's middle row
 // and the norm weight are cached in shared memory (fill_mod_cache).  The sum of squares is the same
-// canonical tree.  Bound by instruction issue and latency: 16 warps (128 registers) measured 63 us at 32768 x 3072
-// mxfp4, 20 took 72 and 24 82 (spills), with one slot each
+// canonical tree.  Bound by instruction issue and latency (70 % of issue slots): 16 warps (128 registers) take 53 us at
+// 32768 x 3072 mxfp4 and 55 us nvfp4, 20 warps 55 and 63, 24 (which spill) 64 and 72, with one slot each
 // (it refills as soon as the row is in registers).
 
 // bf16(h) of one vector, and max |h| (float32, NaN above all) folded into amax.

@@ -251,7 +251,7 @@ int launch_gemm_fp4(const Fp4Gemm& p, const t8g::gemm4::Args& args, int dev, int
   const bool many = (p.M + 255) / 256 * ((p.N + 255) / 256) * 8 > sms;
   if (((p.M > 64 && many) || (p.M > 128 && args.kstages <= 8)) && p.N >= 8) {   // a whole 16-byte piece to store
     // mxfp4 without row or weight scales, as the row operators give it, skips the two products by 1 (9472 x
-    // 8192 x 512: 46 us, 54 with them; x 1024: 50, 58); the gated epilogue spills in that form and keeps them
+    // 8192 x 512: 36 us, 45 with them; x 1024: 43, 48); the gated epilogue spills in that form and keeps them
     if constexpr (MX && OUT != t8g::gemm4::kOutGated) {
       if (!args.xs && !args.ws) return launch_gemm_fp4_pair<MX, OUT, false>(p, args, dev, sms, st);
     }

@@ -244,3 +244,52 @@ def test_no_modulation_row_is_refused():
     with pytest.raises(_lib.T8GError, match="shift is null"):
         ops.rms_mod_quant_fp4(x, none, none, mod_index=torch.zeros(4, dtype=torch.int32, device=DEV))
     assert ops.rms_mod_quant_fp4(none, none, none)[0].shape == (0, 32)
+
+
+# ---------------------------------------------------------------- the given stream
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("form", ["stream", "handle", "default"])
+def test_outputs_belong_to_the_given_stream(kind, form):
+    """A call on a given stream while the current one is far behind: a block that the current stream's work freed but has yet to
+    write is not taken for its outputs, whichever call it is."""
+    g = gen(21)
+    m, n, k = 300, 264, 520
+    x, y, one = randn(g, m, k), randn(g, m, 2 * k), randn(g, 1, k)
+    w = ops.quant_rows_fp4(randn(g, n, k, scale=0.02), kind)
+    res, gate, index = randn(g, m, n), randn(g, 1, n), torch.zeros(m, dtype=torch.int32, device=DEV)
+
+    def calls(stream):
+        q = ops.quant_rows_fp4(x, kind, stream=stream)
+        h = ops.rms_mod_quant_fp4(x, one, one, rows_per_mod=m, kind=kind, stream=stream)
+        hw = ops.rms_mod_quant_fp4(x, one, one, w=one[0], kind=kind, stream=stream)
+        a = ops.swiglu_quant_fp4_fc1(y, kind, stream=stream)
+        b = ops.swiglu_quant_fp4(y[:, :k], y[:, k:], kind, stream=stream)
+        out = [ops.dequant_rows_fp4(*op, kind, stream=stream) for op in (q, h, hw, a, b)]
+        out.append(ops.gemm_fp4(q[0], w[0], q[1], w[1], q[2], w[2], kind=kind, stream=stream))
+        out += [ops.gemm_fp4_gated(q[0], w[0], q[1], w[1], q[2], w[2], None, res, gate, kind=kind, stream=stream, **kw)
+                for kw in (dict(rows_per_gate=m), dict(gate_index=index))]
+        return out
+
+    want = calls(None)
+    torch.cuda.synchronize()
+    current = torch.cuda.Stream()
+    side = torch.cuda.default_stream() if form == "default" else torch.cuda.Stream()
+    given = {"stream": side, "handle": side.cuda_stream, "default": 0}[form]
+    calls(given)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(current):
+        # every size of the outputs, freed while their writing still waits behind a sleep of the current stream
+        sizes = [t.numel() * t.element_size() for t in want] + [m * k // 2, m * 272, m * 4, ops.fp4_scale_bytes(m, k, kind)]
+        blocks = [torch.empty(size, dtype=torch.uint8, device=DEV) for size in sizes for _ in range(4)]
+        torch.cuda._sleep(200_000_000)   # about 0.1 s
+        for t in blocks:
+            t.fill_(0xFF)
+        del blocks, t
+        late = torch.cuda.Event()
+        late.record()
+        got = calls(given)
+    side.synchronize()
+    assert not late.query()   # the calls ran while the current stream slept
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

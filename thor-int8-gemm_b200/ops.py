@@ -7,6 +7,7 @@ stream (default: torch's current stream of the tensor's device).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -492,6 +493,7 @@ def swiglu_quant_tensorwise(gate, up, kind="fp8_e4m3", stream=None):
 # A 4-bit matrix [S, D] is (q, sf, q_scale): q uint8 [S, D / 2], two e2m1 codes a byte (the even column in
 # the low half) at a row pitch that is a multiple of 16 bytes; sf uint8, the block scales in tiles of
 # 128 rows x 4 blocks (`fp4_scale_rows` gives them row by row); q_scale float32 [S], or None (mxfp4).
+# A call with `stream` is as the same call with that stream current: its outputs are that stream's.
 FP4_CODE = {"mxfp4": _lib.QUANT_MXFP4, "nvfp4": _lib.QUANT_NVFP4}
 FP4_BLOCK = {"mxfp4": 32, "nvfp4": 16}
 
@@ -566,7 +568,36 @@ def fp4_scale_rows(sf: torch.Tensor, rows: int, D: int, kind: str) -> torch.Tens
     return t.permute(0, 3, 2, 1, 4).reshape(groups * 128, 4 * words)[:rows, :blocks]
 
 
-def _fp4_empty(S: int, D: int, kind: str, device):
+def _stream_memory(stream, device):
+    """Context for allocating the outputs of a call on `stream`: from the memory that torch keeps for that
+    stream.  A block freed by work on the current stream may still be written there, and an output is not given
+    back to that work while `stream` runs."""
+    if device.type != "cuda":
+        return contextlib.nullcontext()   # the call is refused later
+    if not isinstance(stream, torch.cuda.Stream):
+        handle = int(stream)
+        stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+    return torch.cuda.stream(stream)
+
+
+def _empty(M: int, N: int, dtype: torch.dtype, device, stream) -> torch.Tensor:
+    if stream is not None:
+        with _stream_memory(stream, device):
+            return torch.empty(M, N, dtype=dtype, device=device)
+    return torch.empty(M, N, dtype=dtype, device=device)
+
+
+def _empty_like(t: torch.Tensor, stream) -> torch.Tensor:
+    if stream is not None:
+        with _stream_memory(stream, t.device):
+            return torch.empty_like(t, memory_format=torch.contiguous_format)
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _fp4_empty(S: int, D: int, kind: str, device, stream):
+    if stream is not None:
+        with _stream_memory(stream, device):
+            return _fp4_empty(S, D, kind, device, None)
     if D % 32:
         q = torch.empty(S, -(-D // 32) * 16, dtype=torch.uint8, device=device)[:, :D // 2]
     else:
@@ -628,11 +659,11 @@ def quant_rows_fp4(x: torch.Tensor, kind: str = "nvfp4", stream=None):
     infinity stands for NaN."""
     code = _fp4_code(kind)
     if isinstance(x, torch.Tensor) and x.dim() == 2:
-        out = _fp4_empty(*x.shape, kind, x.device)
+        out = _fp4_empty(*x.shape, kind, x.device, stream)
         if _fp4_launched(_fp4_fast().quant_rows(x, *out, code, _raw(stream))):
             return out
     S, D = _fp4_bf16_rows("x", x)
-    q, sf, q_scale = _fp4_empty(S, D, kind, x.device)
+    q, sf, q_scale = _fp4_empty(S, D, kind, x.device, stream)
     idx = x.get_device()
     _call(_lib.load().t8g_quant_rows_fp4, idx, x.data_ptr(), _pitch(x, S, D, 8), q.data_ptr(), _pitch(q, S, D // 2, 16),
           sf.data_ptr(), _ptr(q_scale), S, D, code, stream)
@@ -646,7 +677,7 @@ def dequant_rows_fp4(q: torch.Tensor, sf: torch.Tensor, q_scale: torch.Tensor | 
     if out_dtype not in OUT_CODE:
         raise TypeError(f"out_dtype {out_dtype} is not one of {tuple(OUT_CODE)}")
     if isinstance(q, torch.Tensor) and q.dim() == 2:
-        out = torch.empty(q.shape[0], 2 * q.shape[1], dtype=out_dtype, device=q.device)
+        out = _empty(q.shape[0], 2 * q.shape[1], out_dtype, q.device, stream)
         if _fp4_launched(_fp4_fast().dequant(q, sf, q_scale, out, OUT_CODE[out_dtype], code, _raw(stream))):
             return out
     S, D = _fp4_operand("q", q, sf, kind)
@@ -659,7 +690,7 @@ def dequant_rows_fp4(q: torch.Tensor, sf: torch.Tensor, q_scale: torch.Tensor | 
             raise ValueError("q_scale must be a contiguous float32 tensor with S elements")
     if sf.get_device() != idx or (q_scale is not None and q_scale.get_device() != idx):
         _one_device(q=q, sf=sf, q_scale=q_scale)
-    out = torch.empty(S, D, dtype=out_dtype, device=q.device)
+    out = _empty(S, D, out_dtype, q.device, stream)
     _call(_lib.load().t8g_dequant_rows_fp4, idx, q.data_ptr(), _pitch(q, S, D // 2, 16), sf.data_ptr(), _ptr(q_scale),
           out.data_ptr(), OUT_CODE[out_dtype], D, S, D, code, stream)
     return out
@@ -672,7 +703,7 @@ def rms_mod_quant_fp4(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor,
     bit, without storing h.  Values of mod_index are trusted to be rows of shift / scale."""
     code = _fp4_code(kind)
     if w is None and mod_index is None and rows_per_mod and isinstance(x, torch.Tensor) and x.dim() == 2:
-        out = _fp4_empty(*x.shape, kind, x.device)
+        out = _fp4_empty(*x.shape, kind, x.device, stream)
         if _fp4_launched(_fp4_fast().rms_mod_quant(x, shift, scale, rows_per_mod, int(scale_is_multiplier), eps, *out, code,
                                                    _raw(stream))):
             return out
@@ -694,7 +725,7 @@ def rms_mod_quant_fp4(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor,
         if w.numel() != D:
             raise ValueError("w must have D elements")
         _one_device(x=x, w=w)
-    q, sf, q_scale = _fp4_empty(S, D, kind, x.device)
+    q, sf, q_scale = _fp4_empty(S, D, kind, x.device, stream)
     _call(_lib.load().t8g_rms_mod_quant_fp4, idx, x.data_ptr(), _pitch(x, S, D, 8), _ptr(w), shift.data_ptr(),
           scale.data_ptr(), _pitch(shift, shift.shape[0], D, 8), _ptr(mod_index), rpm, int(scale_is_multiplier), float(eps),
           q.data_ptr(), _pitch(q, S, D // 2, 16), sf.data_ptr(), _ptr(q_scale), S, D, code, stream)
@@ -714,7 +745,7 @@ def swiglu_quant_fp4(gate: torch.Tensor, up: torch.Tensor, kind: str = "nvfp4", 
 
 def _swiglu_fp4(gate: int, up: int, ld: int, M: int, F: int, kind: str, device, stream):
     code = _fp4_code(kind)
-    q, sf, q_scale = _fp4_empty(M, F, kind, device)
+    q, sf, q_scale = _fp4_empty(M, F, kind, device, stream)
     _call(_lib.load().t8g_swiglu_quant_fp4, device.index, gate, up, ld, q.data_ptr(), _pitch(q, M, F // 2, 16), sf.data_ptr(),
           _ptr(q_scale), M, F, code, stream)
     return q, sf, q_scale
@@ -724,7 +755,7 @@ def swiglu_quant_fp4_fc1(y: torch.Tensor, kind: str = "nvfp4", stream=None):
     """swiglu_quant_fp4 of a [M, 2F] fc1 output whose first half is the gate (read in place)."""
     code = _fp4_code(kind)
     if isinstance(y, torch.Tensor) and y.dim() == 2:
-        out = _fp4_empty(y.shape[0], y.shape[1] // 2, kind, y.device)
+        out = _fp4_empty(y.shape[0], y.shape[1] // 2, kind, y.device, stream)
         if _fp4_launched(_fp4_fast().swiglu_fc1(y, *out, code, _raw(stream))):
             return out
     M, F2 = _fp4_bf16_rows("y", y)
@@ -764,8 +795,11 @@ def _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype)
     return x.get_device(), M, N, K, 0 if w_scale is None else w_scale.numel(), nb
 
 
-def _out_matrix(M: int, N: int, dtype: torch.dtype, device) -> torch.Tensor:
+def _out_matrix(M: int, N: int, dtype: torch.dtype, device, stream) -> torch.Tensor:
     """[M, N] with rows at a multiple of 16 bytes (contiguous when N allows)."""
+    if stream is not None:
+        with _stream_memory(stream, device):
+            return _out_matrix(M, N, dtype, device, None)
     per = 16 // dtype.itemsize
     if N % per == 0:
         return torch.empty(M, N, dtype=dtype, device=device)
@@ -789,14 +823,14 @@ def gemm_fp4(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: torch.T
         raise TypeError(f"out_dtype {out_dtype} is not one of {tuple(OUT_CODE)}")
     fast = out
     if out is None and isinstance(x, torch.Tensor) and isinstance(w, torch.Tensor) and x.dim() == 2 and w.dim() == 2:
-        fast = out = _out_matrix(x.shape[0], w.shape[0], out_dtype, x.device)
+        fast = out = _out_matrix(x.shape[0], w.shape[0], out_dtype, x.device, stream)
     if fast is not None and _fp4_launched(_fp4_fast().gemm(x, w, x_sf, w_sf, x_scale, w_scale, bias, out, out_dtype,
                                                            OUT_CODE[out_dtype], 16 // out_dtype.itemsize, code,
                                                            _raw(stream))):
         return out
     d, M, N, K, nws, nb = _fp4_product_args(x, w, x_sf, w_sf, x_scale, w_scale, bias, kind, out_dtype)
     if out is None:
-        out = _out_matrix(M, N, out_dtype, x.device)
+        out = _out_matrix(M, N, out_dtype, x.device, stream)
     else:
         _need_cuda("out", out, out_dtype, 2)
         if tuple(out.shape) != (M, N):
@@ -819,7 +853,7 @@ def gemm_fp4_gated(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: t
     rows of gate) or m // rows_per_gate; out may be res itself (in-place update)."""
     code = _fp4_code(kind)
     if rows_per_gate and gate_index is None and isinstance(res, torch.Tensor):
-        to = torch.empty_like(res, memory_format=torch.contiguous_format) if out is None else out
+        to = out if out is not None else _empty_like(res, stream)
         if _fp4_launched(_fp4_fast().gated(x, w, x_sf, w_sf, x_scale, w_scale, bias, res, gate, to, rows_per_gate, code,
                                            _raw(stream))):
             return to
@@ -849,7 +883,7 @@ def gemm_fp4_gated(x: torch.Tensor, w: torch.Tensor, x_sf: torch.Tensor, w_sf: t
         if rpg < 1 or (M and (M - 1) // rpg >= gate.shape[0]):
             raise ValueError(f"rows_per_gate={rpg} maps rows past the {gate.shape[0]} gate rows")
     if out is None:
-        out = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
+        out = _empty(M, N, torch.bfloat16, x.device, stream)
     elif out is not res:
         _need_cuda("out", out, torch.bfloat16, 2)
         if tuple(out.shape) != (M, N):

@@ -493,6 +493,7 @@ def swiglu_quant_tensorwise(gate, up, kind="fp8_e4m3", stream=None):
 # A 4-bit matrix [S, D] is (q, sf, q_scale): q uint8 [S, D / 2], two e2m1 codes a byte (the even column in
 # the low half) at a row pitch that is a multiple of 16 bytes; sf uint8, the block scales in tiles of
 # 128 rows x 4 blocks (`fp4_scale_rows` gives them row by row); q_scale float32 [S], or None (mxfp4).
+# The tiles' rows past S are never written nor read into a result: compare operands by `fp4_scale_rows`, not by sf.
 # A call with `stream` is as the same call with that stream current: its outputs are that stream's.
 FP4_CODE = {"mxfp4": _lib.QUANT_MXFP4, "nvfp4": _lib.QUANT_NVFP4}
 FP4_BLOCK = {"mxfp4": 32, "nvfp4": 16}

@@ -16,7 +16,8 @@ dtypes), at run time the op calls the CUDA kernel on the current stream.
     t8g::swiglu_quant(y, kind) -> (q, q_scale)                     (y = [M, 2F] fc1 output)
     t8g::gemm_swiglu(x, w_il, x_scale, w_scale_il, bias_il?) -> act  (fc1 + SwiGLU epilogue)
     t8g::gemm_gated(x, w, x_scale, w_scale, bias?, res, gate, rows_per_gate) -> res + gate * y
-  and of the microscaled 4-bit formats (kind "mxfp4" / "nvfp4"; q_scale is empty for mxfp4):
+  and of the microscaled 4-bit formats (kind "mxfp4" / "nvfp4"; q_scale is empty for mxfp4; the rows of sf's
+  tiles past the last hold whatever the memory held, and reach no result):
     t8g::quant_rows_fp4(x, kind) -> (q, sf, q_scale)
     t8g::rms_mod_quant_fp4(x, shift, scale, w?, mod_index?, rows_per_mod, scale_is_multiplier, eps,
                            kind) -> (q, sf, q_scale)
